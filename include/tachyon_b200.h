@@ -362,6 +362,146 @@ TB_API int tb_sample(tb_context* ctx, const float* logits, float* work, uint32_t
 /* The k largest logits, largest first, lowest index first among equals. idx, val: device [k]. */
 TB_API int tb_topk(tb_context* ctx, const float* logits, uint32_t vocab, uint32_t k, uint32_t* idx, float* val);
 
+/* ---- batched serving: a paged 8-bit key-value cache and what a step does around it (no counterpart in the reference, which
+ * keeps one sequence's f16 cache a model) -------------------------------------------------------------------------------
+ *
+ * A pool of pages, each `page` positions of every key-value head; a request's positions lie in the pages of its row of the
+ * table.  Slot s is position s % page of page s / page.  One scale for a page and key-value head, for keys and values each: 0
+ * (every code is 0) or a power of two; a stored number is code * scale, |code| <= 127.  All words below are device memory
+ * unless they say otherwise; nothing in device memory is trusted: what names no page or lies past the table is skipped.
+ * A step calls tb_page_plan (new lengths, pages and slots), per layer tb_cache_append_q8 and tb_attend_paged_q8 (or
+ * tb_prefill_paged_q8), then tb_logits_adjust in front of a sampler.  Descriptors are checked before the context, so a
+ * descriptor can be tried without a GPU (a good one then fails with "null context").
+ */
+typedef struct tb_pages {
+    int8_t* k;             /* [pages][kv_heads][page][head_dim], 16-byte aligned */
+    int8_t* v;
+    float* k_scale;        /* [pages][kv_heads] */
+    float* v_scale;
+    const uint32_t* table; /* [requests][width]: the page that holds positions page * i ...; only the attention calls read it */
+    uint32_t pages, page;  /* page: 16, 32, 64 or 128 */
+    uint32_t kv_heads, head_dim; /* head_dim: 64, 128, 256 or 512 */
+    uint32_t requests, width;    /* up to 8192 requests; width * page below 2^31 */
+} tb_pages;
+
+/*
+ * Page tables and slot maps from the requests' lengths, without the host knowing them.  Request r has lengths[r] positions in
+ * ceil(lengths[r] / page) pages of its table row and brings fresh[r] new tokens (0: none; TB_REQUEST_ENDS: it is over, its
+ * pages go back and its length becomes 0).  The pages to give are the stack free_pages[0 .. *free_count) followed by the pages
+ * given back (in the order of the requests, then of their positions); new page k, counted over the requests, is the k-th from
+ * that stack's top and goes to the next entry of its request's table row.  What is left of the stack is left in free_pages.
+ * Out: lengths_out (may be lengths), free_count_out (may be free_count), starts[r] = new tokens before request r
+ * ([requests + 1]), and for new token t its slot and position (entries past the last token are left as they were; a slot is
+ * 0xffffffff where the table names no page).  When it cannot be done, *refused says why (TB_PLAN_* bits, 0: done), starts is 0 throughout,
+ * the lengths and the count are the old ones and nothing else is written: pages too few, a length past width * page, more than
+ * max_tokens new tokens, or a free list that would pass `pages` entries.
+ */
+enum { TB_PLAN_PAGES = 1, TB_PLAN_LENGTH = 2, TB_PLAN_TOKENS = 4, TB_PLAN_FREE_LIST = 8 };
+#define TB_REQUEST_ENDS 0xffffffffu
+typedef struct tb_plan {
+    const uint32_t* lengths;
+    const uint32_t* fresh;
+    uint32_t* lengths_out;
+    uint32_t* table;       /* [requests][width] */
+    uint32_t* free_pages;  /* [pages] */
+    const uint32_t* free_count;
+    uint32_t* free_count_out;
+    uint32_t* starts;      /* [requests + 1] */
+    uint32_t* slots;       /* [max_tokens] */
+    uint32_t* positions;   /* [max_tokens] or NULL */
+    uint32_t* refused;
+    uint32_t* scratch;     /* one word, zero before the first launch, left zero */
+    uint32_t requests, width, page, pages, max_tokens;
+} tb_plan;
+TB_API int tb_page_plan(tb_context* ctx, const tb_plan* args);
+
+/*
+ * Rows of keys and values into the cache and out of it.  Token t's row of head h starts at k + t * token_stride + h *
+ * head_stride (values of dtype; strides multiples of 8, so tb_prefill_qkv's caches fit as they are); it belongs to slots[t],
+ * and a slot past the cache is skipped.
+ * tb_cache_append_q8: a page's scale becomes the largest of its old one (0 where the call stores the page's first position) and the least
+ * power of two 2^e >= 2^-126 with max|x| <= 127 * 2^e over its new rows; codes below its first new row are rounded to the new scale, new
+ * ones are x / scale rounded to the nearest (ties to even).  Infinities become +-127 and set no scale, NaN becomes 0.  New rows of one page must be
+ * consecutive tokens in consecutive slots, and no slot may come twice (the outcome is not defined then).
+ * tb_cache_read_q8: the rows' values, code * scale, rounded to dtype.
+ */
+typedef struct tb_cache_rows {
+    tb_pages cache;
+    void* k;               /* read by tb_cache_append_q8, written by tb_cache_read_q8 */
+    void* v;
+    int dtype;             /* TB_F32 or TB_F16 */
+    uint64_t token_stride, head_stride;
+    const uint32_t* slots; /* [tokens] */
+    uint32_t tokens;
+} tb_cache_rows;
+TB_API int tb_cache_append_q8(tb_context* ctx, const tb_cache_rows* args);
+TB_API int tb_cache_read_q8(tb_context* ctx, const tb_cache_rows* args);
+
+/*
+ * Attention over the cache.  Request r's new tokens are rows starts[r] .. starts[r + 1] of q (starts NULL: row r alone), its last
+ * new token sits at position lengths[r] - 1 (keys and values already appended).  A token at position p attends the positions
+ * j <= p, with a window the newest `window` of them; out = softmax(scale q.k) v per query head, heads / kv_heads query heads to a
+ * key-value head.  A token that sees nothing gets zeros; positions whose table entry names no page are not seen.  Rows of q and
+ * out that no request owns, and new tokens of a request past its first `most`, are left as they were.  The same input gives the
+ * same bits; which other requests share the call can change the last ones.
+ * tb_attend_paged_q8: for few rows, most * heads / kv_heads <= 64: a decode step.  f32 accuracy (queries and probabilities are
+ * multiplied in two f16 parts).
+ * tb_prefill_paged_q8: for chunks of a prompt.  Queries and probabilities are rounded to f16 as in tb_prefill_attend.
+ * scratch: tb_paged_scratch_bytes bytes, zero before the first launch; calls may share it as long as they do not overlap
+ * (whatever their shapes).
+ */
+typedef struct tb_paged_attend {
+    tb_pages cache;
+    const void* q;         /* [tokens][heads][head_dim] of q_dtype, q_stride values from token to token */
+    int q_dtype;
+    uint64_t q_stride;     /* a multiple of 8, at least heads * head_dim */
+    const uint32_t* starts;
+    const uint32_t* lengths;
+    uint32_t tokens, heads;
+    uint32_t most;         /* no request brings more new tokens */
+    uint32_t window;       /* 0: none */
+    float scale;
+    void* out;             /* [tokens][heads][head_dim] of out_dtype, out_stride values from token to token */
+    int out_dtype;
+    uint64_t out_stride;
+    void* scratch;
+    size_t scratch_bytes;
+} tb_paged_attend;
+TB_API size_t tb_paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim);
+TB_API int tb_attend_paged_q8(tb_context* ctx, const tb_paged_attend* args);
+TB_API int tb_prefill_paged_q8(tb_context* ctx, const tb_paged_attend* args);
+
+/*
+ * Logits of a batch made ready for a sampler (tb_sample, tb_topk): out[r][t] from x = logits[r][t], each part optional (NULL):
+ *   token t in history[r][0 .. total[r]):           x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   c = its count in history[r][prompt[r] .. total[r]): x -= c > 0 ? frequency[r] * c + presence[r] : 0
+ *   bias_token[r][i] == t, i < bias_count[r]:        x += bias[r][i], in the order of i (summed first when a token comes twice)
+ *   mask m = mask_of[r] (NULL: r), bit t clear:      x = -inf (also over NaN); m >= masks: no mask.  A mask may let nothing through: the row is -inf.
+ * f32 arithmetic, rounded once to dtype.  Tokens past the vocabulary in history and biases are ignored.  out may be logits.
+ */
+typedef struct tb_logits {
+    const void* logits;    /* [rows][vocab], stride values from row to row */
+    void* out;
+    int dtype;             /* TB_F32 or TB_F16, of both */
+    uint32_t rows, vocab;
+    uint64_t stride, out_stride;
+    const uint32_t* history; /* [rows][history_stride]: the prompt's tokens, then the generated ones */
+    uint32_t history_stride;
+    const uint32_t* prompt;  /* [rows] */
+    const uint32_t* total;   /* [rows] */
+    const float* repetition; /* [rows] or NULL, as the next two */
+    const float* frequency;
+    const float* presence;
+    const uint32_t* bias_token; /* [rows][bias_stride] */
+    const float* bias;
+    const uint32_t* bias_count; /* [rows] */
+    uint32_t bias_stride;
+    const uint32_t* allowed; /* [masks][allowed_stride] words of 32 tokens */
+    const uint32_t* mask_of; /* [rows] or NULL */
+    uint32_t allowed_stride, masks;
+} tb_logits;
+TB_API int tb_logits_adjust(tb_context* ctx, const tb_logits* args);
+
 /* Seeded synthetic tensors (this build's generators; the reference's benches are synthetic too, benches/gemv.rs:8-9). */
 TB_API int tb_fill_codes(tb_context* ctx, uint64_t seed, uint64_t stream_id, int8_t* dev, size_t n);
 TB_API int tb_fill_scales(tb_context* ctx, uint64_t seed, uint64_t stream_id, uint16_t* dev, size_t n, float mul);

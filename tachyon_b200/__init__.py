@@ -13,9 +13,11 @@ import os
 import numpy as np
 
 from . import _lib
-from ._lib import Attend, Config, EncoderConfig, Load, Loaded, Settings
+from ._lib import Attend, CacheRows, Config, EncoderConfig, Load, Loaded, Logits, PagedAttend, PagePlan, Pages, Settings
 
 F32, F16 = 0, 1
+REQUEST_ENDS = 0xFFFFFFFF  # PagePlan.fresh of a request that is over
+PLAN_PAGES, PLAN_LENGTH, PLAN_TOKENS, PLAN_FREE_LIST = 1, 2, 4, 8  # why PagePlan.refused is not 0
 
 
 class Error(RuntimeError):
@@ -284,6 +286,34 @@ class Context:
 
     def topk(self, logits, vocab, k, idx, val) -> None:
         check(self.lib.tb_topk(self.handle, logits.ptr, vocab, k, idx.ptr, val.ptr))
+
+    # ---- batched serving over a paged 8-bit cache (one launch each) ----
+    def page_plan(self, args: PagePlan) -> None:
+        """tb_page_plan: new lengths, page tables, slots and positions from the requests' lengths."""
+        check(self.lib.tb_page_plan(self.handle, C.byref(args)))
+
+    def cache_append_q8(self, args: CacheRows) -> None:
+        """tb_cache_append_q8: rows of keys and values into their slots, quantised."""
+        check(self.lib.tb_cache_append_q8(self.handle, C.byref(args)))
+
+    def cache_read_q8(self, args: CacheRows) -> None:
+        """tb_cache_read_q8: the values that slots hold."""
+        check(self.lib.tb_cache_read_q8(self.handle, C.byref(args)))
+
+    def paged_scratch_bytes(self, head_dim: int) -> int:
+        return self.lib.tb_paged_scratch_bytes(self.handle, head_dim)
+
+    def attend_paged_q8(self, args: PagedAttend) -> None:
+        """tb_attend_paged_q8: one or a few new tokens of every request over the cache."""
+        check(self.lib.tb_attend_paged_q8(self.handle, C.byref(args)))
+
+    def prefill_paged_q8(self, args: PagedAttend) -> None:
+        """tb_prefill_paged_q8: chunks of prompts over the cache."""
+        check(self.lib.tb_prefill_paged_q8(self.handle, C.byref(args)))
+
+    def logits_adjust(self, args: Logits) -> None:
+        """tb_logits_adjust: penalties, biases and masks on a batch of logits."""
+        check(self.lib.tb_logits_adjust(self.handle, C.byref(args)))
 
 
 class Event:

@@ -23,6 +23,36 @@ class Attend(C.Structure):
     ]
 
 
+class Pages(C.Structure):
+    """tb_pages: a paged 8-bit key-value cache, one scale for a page and key-value head."""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("table", vp), ("pages", u32), ("page", u32), ("kv_heads", u32), ("head_dim", u32),
+                ("requests", u32), ("width", u32)]
+
+
+class PagePlan(C.Structure):
+    """tb_plan: page tables and slot maps from the requests' lengths."""
+    _fields_ = [("lengths", vp), ("fresh", vp), ("lengths_out", vp), ("table", vp), ("free_pages", vp), ("free_count", vp), ("free_count_out", vp), ("starts", vp),
+                ("slots", vp), ("positions", vp), ("refused", vp), ("scratch", vp), ("requests", u32), ("width", u32), ("page", u32), ("pages", u32), ("max_tokens", u32)]
+
+
+class CacheRows(C.Structure):
+    """tb_cache_rows: rows of keys and values and the slots they belong to."""
+    _fields_ = [("cache", Pages), ("k", vp), ("v", vp), ("dtype", i32), ("token_stride", u64), ("head_stride", u64), ("slots", vp), ("tokens", u32)]
+
+
+class PagedAttend(C.Structure):
+    """tb_paged_attend: attention of new tokens over a paged 8-bit cache."""
+    _fields_ = [("cache", Pages), ("q", vp), ("q_dtype", i32), ("q_stride", u64), ("starts", vp), ("lengths", vp), ("tokens", u32), ("heads", u32), ("most", u32),
+                ("window", u32), ("scale", f32), ("out", vp), ("out_dtype", i32), ("out_stride", u64), ("scratch", vp), ("scratch_bytes", sz)]
+
+
+class Logits(C.Structure):
+    """tb_logits: penalties, biases and masks on a batch of logits."""
+    _fields_ = [("logits", vp), ("out", vp), ("dtype", i32), ("rows", u32), ("vocab", u32), ("stride", u64), ("out_stride", u64), ("history", vp),
+                ("history_stride", u32), ("prompt", vp), ("total", vp), ("repetition", vp), ("frequency", vp), ("presence", vp), ("bias_token", vp), ("bias", vp),
+                ("bias_count", vp), ("bias_stride", u32), ("allowed", vp), ("mask_of", vp), ("allowed_stride", u32), ("masks", u32)]
+
+
 class Config(C.Structure):
     _fields_ = [
         ("hidden", u32), ("ffn", u32), ("heads", u32), ("kv_heads", u32), ("head_dim", u32), ("vocab", u32), ("layers", u32), ("window", u32),
@@ -130,6 +160,13 @@ SIGNATURES = {
     "tb_attend_512_scratch_bytes": (C.c_size_t, [u32, u32]),
     "tb_sample_greedy": (i32, [vp, vp, u32, f32, f32, vp, vp, vp, vp, vp]),
     "tb_topk": (i32, [vp, vp, u32, u32, vp, vp]),
+    "tb_page_plan": (i32, [vp, C.POINTER(PagePlan)]),
+    "tb_cache_append_q8": (i32, [vp, C.POINTER(CacheRows)]),
+    "tb_cache_read_q8": (i32, [vp, C.POINTER(CacheRows)]),
+    "tb_paged_scratch_bytes": (sz, [vp, u32]),
+    "tb_attend_paged_q8": (i32, [vp, C.POINTER(PagedAttend)]),
+    "tb_prefill_paged_q8": (i32, [vp, C.POINTER(PagedAttend)]),
+    "tb_logits_adjust": (i32, [vp, C.POINTER(Logits)]),
     "tb_fill_codes": (i32, [vp, u64, u64, vp, sz]),
     "tb_fill_scales": (i32, [vp, u64, u64, vp, sz, f32]),
     "tb_fill_gauss_f16": (i32, [vp, u64, u64, vp, sz, f32]),
