@@ -418,7 +418,7 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
     PagedArgs a{};
     a.k = c.k, a.v = c.v, a.ks = c.k_scale, a.vs = c.v_scale, a.table = c.table, a.pages = c.pages, a.shift = log2_of(c.page), a.kv_heads = c.kv_heads;
     a.requests = c.requests, a.width = c.width, a.q = p.q, a.q_stride = p.q_stride, a.q_f16 = p.q_dtype == TB_F16, a.starts = p.starts, a.lengths = p.lengths;
-    a.tokens = p.tokens, a.heads = p.heads, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window, a.least = 4;
+    a.tokens = p.tokens, a.heads = p.heads, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window > 0x7fffffffu ? 0 : p.window, a.least = 4;
     a.scale = p.scale * 1.4426950408889634f, a.out = p.out, a.out_stride = p.out_stride, a.out_f16 = p.out_dtype == TB_F16;
     a.count = static_cast<uint32_t*>(p.scratch);
     a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.scratch) + COUNT_BYTES);
@@ -453,6 +453,7 @@ extern "C" int tb_prefill_paged_q8(tb_context* ctx, const tb_paged_attend* args)
     return entry([&] {
         TB_TRY(check_attend(args, "tb_prefill_paged_q8", false));
         if (!ctx) return fail(OUT_OF_RANGE, "null context");
-        return args->tokens == 0 ? (int)OK : launch_attend_paged(ctx, *args);
+        if (args->tokens == 0) return (int)OK;
+        return prefill_paged_supports(*args) ? launch_prefill_paged(ctx, *args) : launch_attend_paged(ctx, *args);
     });
 }

@@ -500,6 +500,12 @@ def test_attend_gives_the_same_bits_and_shares_scratch(ctx):
     assert rng is not None
 
 
+@pytest.mark.parametrize("window", [0x7FFFFFFF, 0x80000000, 0xFFFFFFFF])
+def test_attend_windows_past_every_position(ctx, window):
+    attend_case(ctx, 64, 16, 1, 2, [100, 7], [2, 1], window, np.float16, np.float32)
+    attend_case(ctx, 64, 16, 1, 2, [100, 7], [90, 1], window, np.float16, np.float32, prefill=True)
+
+
 def test_attend_needs_its_scratch(ctx):
     cache = Cache(ctx, 2, 1, 16, 64, 1)
     small = ctx.zeros(ctx.paged_scratch_bytes(64) - 16)
