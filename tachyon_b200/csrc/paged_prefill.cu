@@ -4,14 +4,14 @@
 // positions that start at multiples of KT.  Everything the tensor cores read of the queries' side stays in tensor memory: the
 // queries (stored once), the scores S = Q K^T (two buffers), the probabilities (f16, over the scores they came from) and the
 // output, so shared memory only carries keys and values: codes turned to f16 on the way in, a byte read where the f16 cache's
-// kernel reads two.  Fourteen warps:
-//   warps 0-3    a thread a query row: scores out of tensor memory, maximum, exponentials, probabilities back into it; the running
-//                maximum moves only when a tile passes it by 2^8, and only then the output is rescaled;
-//   warps 4-11   codes to f16: 16 codes a thread and turn, loaded a tile ahead, as 0x6400 | (code + 128) by byte permutes and one packed
+// kernel reads two.  Eighteen warps:
+//   warps 0-7    softmax, two threads a query row, half of a tile's keys each: scores out of tensor memory, maximum (the two trade theirs
+//                through shared memory), exponentials, probabilities back into it; the running maximum moves only when a tile passes it by 2^8, and only then the output is rescaled;
+//   warps 8-15   codes to f16: 16 codes a thread and turn, loaded a tile ahead, as 0x6400 | (code + 128) by byte permutes and one packed
 //                fused multiply-add (x * f - 1152 f, exact), stored in the 128-byte swizzle; keys K-major, values as they lie in
 //                the cache, which is the MN-major form of a B operand;
-//   warp 12      one thread issues the products, S of tile i + 1 ahead of P V of tile i;
-//   warp 13      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
+//   warp 16      one thread issues the products, S of tile i + 1 ahead of P V of tile i;
+//   warp 17      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
 // A page's scales are powers of two.  Keys carry theirs relative to the tile's largest, which multiplies the scores; values theirs
 // relative to the largest scale met so far, which multiplies the output at the end (and rescales it when it grows).  Every wait is bounded.
 #include "common.cuh"
@@ -24,7 +24,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int ROWS = 128, CONVERT_WARPS = 8, THREADS = 14 * 32, AHEAD = 4, MOST_PAGES = 8;
+constexpr int ROWS = 128, SOFT_WARPS = 8, CONVERT_WARPS = 8, GROUP_WARPS = CONVERT_WARPS / 4, MMA_WARP = SOFT_WARPS + CONVERT_WARPS, THREADS = (MMA_WARP + 2) * 32, AHEAD = 8, MOST_PAGES = 8;
 
 template <int D>
 struct Shape {
@@ -33,16 +33,16 @@ struct Shape {
     static constexpr int STAGE = D / 64 * KCH;                // a tile's keys (or values)
     static constexpr int OFF_V = 2 * STAGE, OFF_SUM = 4 * STAGE;
     static constexpr int COL_O = 0, COL_S = D, COL_Q = D + 2 * KT;  // tensor-memory columns
-    static constexpr uint32_t UNITS = KT * (D / 16) / (CONVERT_WARPS * 32);  // sixteen codes each, a thread and tile
+    static constexpr uint32_t UNITS = KT * (D / 16) / (GROUP_WARPS * 32);  // sixteen codes each, a thread and tile
     // kind::f16, f32 accumulator, A from tensor memory; N >> 3 at bit 17, M >> 4 at bit 24, bit 16: B is MN-major.
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     static_assert(COL_Q + D / 2 <= 512, "tensor memory has 512 columns");
 };
 
-struct Ahead {  // what warp 13 finds out about a tile
-    uint32_t id[MOST_PAGES];             // 0xffffffff: no page
-    uint32_t kf[MOST_PAGES], vf[MOST_PAGES];  // factors, two f16 each
+struct Ahead {  // what the last warp finds out about a tile
+    unsigned long long at[MOST_PAGES];   // where the page's first code of the tile lies (page 0 where there is no page: its factors are 0)
+    uint2 kf[MOST_PAGES], vf[MOST_PAGES];  // a page's factor f and -1152 f, two f16 each
     uint32_t keys[4];                    // bit c: key c of the tile has a page
     float kref, shrink;                  // multiplies the scores; what the output is multiplied by before this tile
 };
@@ -53,6 +53,7 @@ struct Shared {
     float vref;
     Ahead ahead[AHEAD];
     uint32_t part[THREADS / 32];
+    float xch[2][2][ROWS];  // [tile's parity][half][row]: what a row's two threads trade: each tile their maxima, at the end their sums
 };
 
 struct PrefillArgs {
@@ -71,12 +72,20 @@ struct PrefillArgs {
     int q_f16, out_f16;
 };
 
-// D = A B with A in tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// D = A B with A in tensor memory, and the commit of what was issued; the whole warp calls them, the thread with `leader` issues.  Run by
+// one lane under a branch, every product first moves its operands to uniform registers: 75 clocks each instead of the product's own time.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_by(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -85,21 +94,52 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
         "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// 32 columns of this thread's lane, there when the statement is done.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+        "%26, %27, %28, %29, %30, %31"
+        "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// 64 columns of this thread's lane, there when the statement is done.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+        "%26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, "
+        "%50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+        "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+          "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]),
+          "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]),
+          "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Sixteen codes as f16 times a factor: two 16-byte pieces.
-__device__ __forceinline__ void convert16(const uint4& w, uint32_t factor, uint4 (&out)[2]) {
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-    const __half2 f = *reinterpret_cast<const __half2*>(&factor);
-    const __half2 off = __hmul2(f, __half2half2(__ushort_as_half(0xe480)));  // -1152 f
-    uint32_t r[8];
+// Eight codes as f16 times a factor (f, -1152 f): a 16-byte piece.
+__device__ __forceinline__ uint4 convert8(uint32_t a, uint32_t b, const uint2& factor) {
+    const __half2 f = *reinterpret_cast<const __half2*>(&factor.x), off = *reinterpret_cast<const __half2*>(&factor.y);
+    uint4 out;
+    uint32_t* r = &out.x;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t b = words[i] ^ 0x80808080u, lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
+    for (int i = 0; i < 2; i++) {
+        const uint32_t w = (i ? b : a) ^ 0x80808080u, lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
         const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&lo), f, off), y = __hfma2(*reinterpret_cast<const __half2*>(&hi), f, off);
         r[2 * i] = *reinterpret_cast<const uint32_t*>(&x), r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
     }
-    out[0] = make_uint4(r[0], r[1], r[2], r[3]), out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    return out;
 }
 
 template <int D>
@@ -160,13 +200,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     const uint32_t nt = end > tile0 ? (end - tile0 + KT - 1) / KT : 0;
 
     if (th == 0) {
-        mbar_init(&sh.q_full, 4), mbar_init(&sh.drained, 1);
-        for (int i = 0; i < 2; i++) mbar_init(&sh.k_full[i], CONVERT_WARPS), mbar_init(&sh.v_full[i], CONVERT_WARPS), mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_ready[i], 4);
+        mbar_init(&sh.q_full, SOFT_WARPS), mbar_init(&sh.drained, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&sh.k_full[i], GROUP_WARPS), mbar_init(&sh.v_full[i], GROUP_WARPS), mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_ready[i], SOFT_WARPS);
         for (int i = 0; i < AHEAD; i++) mbar_init(&sh.pv_done[i], 1), mbar_init(&sh.known[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -183,12 +223,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         }
     };
 
-    if (warp < 4) {
-        // ---- queries, softmax, output: this thread has row `row`, tensor-memory lane of the same number -------------------
-        const uint32_t row = row0 + th, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
+    if (warp < SOFT_WARPS) {
+        // ---- queries, softmax, output: a query row's two threads (warps w and w + 4, tensor-memory lane = row) take half of a tile's
+        // keys and half of the dimensions each ---------------------------------------------------------------------------
+        constexpr int HK = KT / 2, HD = D / 2;
+        const uint32_t quarter = warp & 3, half = warp >> 2, me = 32 * quarter + lane;
+        const uint32_t row = row0 + me, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
         const bool valid = tok < n;
-        const uint32_t lanes = tmem + ((32 * warp) << 16);
-        const unsigned long long q_at = (unsigned long long)(first + tok) * a.q_stride + (unsigned long long)head * D;
+        const uint32_t lanes = tmem + ((32 * quarter) << 16);
+        const unsigned long long q_at = (unsigned long long)(first + tok) * a.q_stride + (unsigned long long)head * D + half * HD;
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (int)quarter) : "memory"); };  // the row's two warps
         // The row is scaled by a power of two so that its largest lies in [1, 2): f16 then loses 2^-11 of it whatever its size.
         float factor = 0.0f;
         if (nt != 0) {
@@ -211,16 +255,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                 }
             };
             float big = 0.0f;
-            for (int d = 0; d < D; d += 8) {
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
                 float x[8];
                 eight(d, x);
 #pragma unroll
                 for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
             }
+            sh.xch[1][half][me] = big;
+            meet();
+            big = fmaxf(big, sh.xch[1][half ^ 1][me]);
             const uint32_t expo = min(max(__float_as_uint(big) >> 23, 1u), 253u);
             const float inv = __uint_as_float((254u - expo) << 23);
             factor = a.scale * __uint_as_float(expo << 23);
-            for (int c = 0; c < D / 32; c++) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; c++) {
                 uint32_t h[16];
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
@@ -232,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                         h[g * 4 + e] = *reinterpret_cast<const uint32_t*>(&v);
                     }
                 }
-                tmem_store16(lanes + S::COL_Q + c * 16, h);
+                tmem_store16(lanes + S::COL_Q + half * (HD / 2) + c * 16, h);
             }
             tmem_wait_st();
         }
@@ -247,73 +296,67 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
             const uint32_t buf = i & 1, sbuf = lanes + S::COL_S + buf * KT;
             const Ahead& info = sh.ahead[i % AHEAD];
             wait(&sh.known[i % AHEAD], (i / AHEAD) & 1);
+            const float f = info.kref * factor, shrink = info.shrink;
+            // Key j0 + c is seen when lo <= c < hi and it has a page.
+            const int j0 = (int)(tile0 + i * KT + half * HK), lo = oldest - j0, hi = p + 1 - j0;
+            bool all = lo <= 0 && hi >= HK;
+            uint32_t keys[HK / 32];
+#pragma unroll
+            for (int c = 0; c < HK / 32; c++) keys[c] = info.keys[half * (HK / 32) + c], all = all && keys[c] == 0xffffffffu;
+            all = __all_sync(0xffffffffu, all);
             wait(&sh.s_full[buf], (i >> 1) & 1);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float f = info.kref * factor, shrink = info.shrink;
-            const int j0 = (int)(tile0 + i * KT);
-            float mt = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < KT / 32; c++) {
-                uint32_t s[32];
-                tmem_load32(sbuf + c * 32, s);
-                const int lo = oldest - (j0 + 32 * c), hi = p + 1 - (j0 + 32 * c);
-                const uint32_t keys = info.keys[c];
-                if (__all_sync(0xffffffffu, lo <= 0 && hi >= 32) && keys == 0xffffffffu) {
+            uint32_t s[HK];
+            tmem_load(sbuf + half * HK, s);
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!all) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) mt = fmaxf(mt, __uint_as_float(s[e]));
-                } else {
+                for (int c = 0; c < HK / 32; c++)
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (e >= lo && e < hi && ((keys >> e) & 1u)) mt = fmaxf(mt, __uint_as_float(s[e]));
-                }
+                        if (!(32 * c + e >= lo && 32 * c + e < hi && ((keys[c] >> e) & 1u))) s[32 * c + e] = 0xff800000u;  // -inf
             }
-            mt *= f;
+#pragma unroll
+            for (int e = 0; e < HK; e++) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[e]));
+            float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            sh.xch[buf][half][me] = mt;
+            meet();  // also: both have read their scores, so the probabilities may go over them
+            mt = fmaxf(mt, sh.xch[buf][half ^ 1][me]);
+            mt = mt == -INFINITY ? mt : mt * f;  // f may be 0
             float corr = shrink;
             if (mt > m_used + 8.0f) {  // also a row's first keys (m_used = -inf)
-                corr = ex2(m_used - mt);
-                l_run *= corr;
-                corr *= shrink;
+                const float turn = ex2(m_used - mt);
+                l_run *= turn;
+                corr *= turn;
                 m_used = mt;
             }
             const float base = fmaxf(m_used, -1e30f);  // finite: a row that has seen nothing yet gets 2^-inf = 0 and no NaN
-            float sum = 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < KT / 32; c++) {
-                uint32_t s[32], h[16];
-                tmem_load32(sbuf + c * 32, s);
-                const int lo = oldest - (j0 + 32 * c), hi = p + 1 - (j0 + 32 * c);
-                const uint32_t keys = info.keys[c];
-                if (__all_sync(0xffffffffu, lo <= 0 && hi >= 32) && keys == 0xffffffffu) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float e0 = ex2(fmaf(__uint_as_float(s[2 * e]), f, -base)), e1 = ex2(fmaf(__uint_as_float(s[2 * e + 1]), f, -base));
-                        sum += e0 + e1;
-                        const __half2 v = __floats2half2_rn(e0, e1);
-                        h[e] = *reinterpret_cast<const uint32_t*>(&v);
-                    }
-                } else {
-                    auto one = [&](int e) { return e >= lo && e < hi && ((keys >> e) & 1u) ? ex2(fmaf(__uint_as_float(s[e]), f, -base)) : 0.0f; };
+            for (int c = 0; c < HK / 32; c++) {
+                uint32_t h[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float e0 = one(2 * e), e1 = one(2 * e + 1);
-                        sum += e0 + e1;
-                        const __half2 v = __floats2half2_rn(e0, e1);
-                        h[e] = *reinterpret_cast<const uint32_t*>(&v);
-                    }
+                for (int e = 0; e < 16; e++) {
+                    float e0 = ex2(fmaf(__uint_as_float(s[32 * c + 2 * e]), f, -base)), e1 = ex2(fmaf(__uint_as_float(s[32 * c + 2 * e + 1]), f, -base));
+                    if (!all && f == 0.0f) e0 = s[32 * c + 2 * e] == 0xff800000u ? 0.0f : e0, e1 = s[32 * c + 2 * e + 1] == 0xff800000u ? 0.0f : e1;  // -inf * 0
+                    sum[e & 3] += e0 + e1;
+                    const __half2 v = __floats2half2_rn(e0, e1);
+                    h[e] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                tmem_store16(sbuf + c * 16, h);  // over scores this row has done with
+                tmem_store16(sbuf + (half * (HK / 32) + c) * 16, h);
             }
-            l_run += sum;
+            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if (i > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
                 wait(&sh.pv_done[(i - 1) % AHEAD], ((i - 1) / AHEAD) & 1);  // the output must be at rest
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
+                for (int c = 0; c < HD / 32; c++) {
                     uint32_t o[32];
-                    tmem_load32(lanes + S::COL_O + c * 32, o);
+                    const uint32_t at = lanes + S::COL_O + half * HD + c * 32;
+                    tmem_load(at, o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                    tmem_store32(lanes + S::COL_O + c * 32, o);
+                    tmem_store32(at, o);
                 }
             }
             tmem_wait_st();
@@ -323,13 +366,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         }
         if (nt != 0) wait(&sh.pv_done[(nt - 1) % AHEAD], ((nt - 1) / AHEAD) & 1);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        sh.xch[nt & 1][half][me] = l_run;  // not the slots of the last tile, which the other warp may still read
+        meet();
+        l_run += sh.xch[nt & 1][half ^ 1][me];
         if (ok) {
             const float inv = l_run > 0.0f || l_run != l_run ? sh.vref / l_run : 0.0f;
-            const unsigned long long out_at = (unsigned long long)(first + tok) * a.out_stride + (unsigned long long)head * D;
+            const unsigned long long out_at = (unsigned long long)(first + tok) * a.out_stride + (unsigned long long)head * D + half * HD;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; c++) {
+            for (int c = 0; c < HD / 32; c++) {
                 uint32_t o[32];
-                if (nt != 0) tmem_load32(lanes + S::COL_O + c * 32, o);
+                if (nt != 0) tmem_load(lanes + S::COL_O + half * HD + c * 32, o);
                 if (valid) {
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = nt == 0 || inv == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
@@ -354,140 +400,149 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                 __syncwarp();
             }
         }
-    } else if (warp < 4 + CONVERT_WARPS) {
+    } else if (warp < MMA_WARP) {
         // ---- codes to f16 ----------------------------------------------------------------------------------------------
-        const uint32_t me = th - 128;
-        constexpr uint32_t PER_ROW = D / 16, UNITS = S::UNITS;
-        uint4 kw[UNITS], vw[UNITS];
-        // Unit u of this thread: key (me + 256 u) / PER_ROW of the tile, its codes 16 ((me + 256 u) % PER_ROW) ...
-        auto load = [&](const int8_t* codes, const Ahead& info, uint32_t i, uint4 (&w)[UNITS]) {
-            const uint32_t j0 = tile0 + i * KT;
-#pragma unroll
-            for (uint32_t u = 0; u < UNITS; u++) {
-                const uint32_t x = me + u * (CONVERT_WARPS * 32), key = x / PER_ROW, c = x % PER_ROW;
-                const uint32_t id = info.id[((j0 + key) >> a.shift) - (j0 >> a.shift)];
-                w[u] = make_uint4(0, 0, 0, 0);
-                if (id != 0xffffffffu) {
-                    const int8_t* p = codes + ((((size_t)id * a.kv_heads + kvh) << a.shift) + ((j0 + key) & ((1u << a.shift) - 1))) * D + c * 16;
-                    w[u] = __ldg(reinterpret_cast<const uint4*>(p));
-                }
-            }
-        };
-        auto store = [&](uint8_t* stage, const Ahead& info, const uint32_t* factors, uint32_t i, const uint4 (&w)[UNITS]) {
-            const uint32_t j0 = tile0 + i * KT;
-#pragma unroll
-            for (uint32_t u = 0; u < UNITS; u++) {
-                const uint32_t x = me + u * (CONVERT_WARPS * 32), key = x / PER_ROW, c = x % PER_ROW;
-                const uint32_t factor = factors[((j0 + key) >> a.shift) - (j0 >> a.shift)];
-                uint4 out[2];
-                convert16(w[u], factor, out);
-                uint8_t* box = stage + (c >> 2) * S::KCH + key * 128;
-                const uint32_t flip = (c >> 2) & 1;  // neighbours four codes' boxes apart start with different halves: no bank twice in a quarter warp
-                const uint32_t piece = (c & 3) * 2;
-                *reinterpret_cast<uint4*>(box + (((piece + flip) ^ (key & 7)) << 4)) = flip ? out[1] : out[0];
-                *reinterpret_cast<uint4*>(box + (((piece + (flip ^ 1)) ^ (key & 7)) << 4)) = flip ? out[0] : out[1];
-            }
-        };
-        if (nt != 0) {
-            wait(&sh.known[0], 0);
-            load(a.k, sh.ahead[0], 0, kw);
-            load(a.v, sh.ahead[0], 0, vw);
-        }
-        for (uint32_t i = 0; i < nt; i++) {
-            const uint32_t buf = i & 1;
+        // Four groups of two warps: keys of the even tiles, values of the even ones, keys of the odd ones, values of the odd ones.  The fence
+        // in front of the tensor cores waits for a warp's loads in flight as well, so a warp asks for its next tile behind it and the
+        // groups cover each other's trips to the L2.
+        // Unit u of a thread: sixteen codes 64 box + 16 part ... of key key0 + STEP u.  Eight neighbouring lanes take four parts of two
+        // keys, so their 16-byte pieces meet no bank twice.
+        constexpr uint32_t UNITS = S::UNITS, BOXES = D / 64, STEP = GROUP_WARPS * 32 * 16 / D;
+        const uint32_t group = (warp - SOFT_WARPS) / GROUP_WARPS, odd = group >> 1;
+        const bool values = group & 1;
+        const uint32_t me = (th - SOFT_WARPS * 32) % (GROUP_WARPS * 32), part = me & 3, box = (me >> 3) & (BOXES - 1), key0 = (me >> 3) / BOXES * 2 + ((me >> 2) & 1);
+        const int8_t* codes = (values ? a.v : a.k) + box * 64 + part * 16;
+        uint8_t* stage = raw + (values ? S::OFF_V : 0) + odd * S::STAGE + box * S::KCH + key0 * 128;
+        const uint32_t to0 = ((part * 2) ^ (key0 & 7)) << 4, to1 = ((part * 2 + 1) ^ (key0 & 7)) << 4;
+        uint64_t* full = (values ? sh.v_full : sh.k_full) + odd;
+        const uint32_t mask = min(1u << a.shift, (uint32_t)KT) - 1, shift = min(a.shift, (uint32_t)(KT == 64 ? 6 : 7));  // a page's part of a tile
+        uint4 w[UNITS];
+        auto load = [&](uint32_t i) {
             const Ahead& info = sh.ahead[i % AHEAD];
-            if (i >= 2) wait(&sh.s_full[buf], ((i - 2) >> 1) & 1);  // S of the tile two before has read this buffer
-            store(raw + buf * S::STAGE, info, info.kf, i, kw);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.k_full[buf]);
-            const bool more = i + 1 < nt;
-            if (more) {
-                wait(&sh.known[(i + 1) % AHEAD], ((i + 1) / AHEAD) & 1);
-                load(a.k, sh.ahead[(i + 1) % AHEAD], i + 1, kw);
+            wait(&sh.known[i % AHEAD], (i / AHEAD) & 1);
+#pragma unroll
+            for (uint32_t u = 0; u < UNITS; u++) {
+                const uint32_t key = key0 + u * STEP;
+                w[u] = __ldg(reinterpret_cast<const uint4*>(codes + info.at[key >> shift] + (key & mask) * D));
             }
-            if (i >= 2) wait(&sh.pv_done[(i - 2) % AHEAD], ((i - 2) / AHEAD) & 1);
-            store(raw + S::OFF_V + buf * S::STAGE, info, info.vf, i, vw);
+        };
+        if (odd < nt) load(odd);
+        for (uint32_t i = odd; i < nt; i += 2) {
+            // S (or P V) of the tile two before has read this buffer.
+            if (i >= 2) wait(values ? &sh.pv_done[(i - 2) % AHEAD] : &sh.s_full[odd], values ? ((i - 2) / AHEAD) & 1 : ((i - 2) >> 1) & 1);
+            const uint2* factors = values ? sh.ahead[i % AHEAD].vf : sh.ahead[i % AHEAD].kf;
+#pragma unroll
+            for (uint32_t u = 0; u < UNITS; u++) {
+                const uint2 f = factors[(key0 + u * STEP) >> shift];
+                const uint32_t flip = STEP == 4 && (u & 1) ? 64 : 0;  // four keys on, the swizzle's upper bit turns
+                *reinterpret_cast<uint4*>(stage + (to0 ^ flip) + u * STEP * 128) = convert8(w[u].x, w[u].y, f);
+                *reinterpret_cast<uint4*>(stage + (to1 ^ flip) + u * STEP * 128) = convert8(w[u].z, w[u].w, f);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.v_full[buf]);
-            if (more) load(a.v, sh.ahead[(i + 1) % AHEAD], i + 1, vw);
+            if (lane == 0) mbar_arrive(full);
+            if (i + 2 < nt) load(i + 2);
         }
-    } else if (warp == 12) {
+    } else if (warp == MMA_WARP) {
         // ---- products --------------------------------------------------------------------------------------------------
-        if (lane == 0 && nt != 0) {
-            const uint32_t ka = smem_addr(raw), va = smem_addr(raw + S::OFF_V);
+        if (nt != 0) {
+            const uint32_t leader = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t k_desc = desc_k_major(smem_addr(raw)), v_desc = desc_mn_major(smem_addr(raw + S::OFF_V), S::KCH);  // addresses count in 16 bytes
+            auto all_wait = [&](uint64_t* bar, uint32_t parity) {
+                wait(bar, parity);
+                ok = __all_sync(0xffffffffu, ok);
+            };
             auto scores = [&](uint32_t i) {
-                wait(&sh.k_full[i & 1], (i >> 1) & 1);
+                all_wait(&sh.k_full[i & 1], (i >> 1) & 1);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t desc = k_desc + (i & 1) * (S::STAGE >> 4);
+                const uint32_t d = tm + S::COL_S + (i & 1) * KT;
 #pragma unroll
-                for (int k = 0; k < D / 16; k++)
-                    mma_ts(tmem + S::COL_S + (i & 1) * KT, tmem + S::COL_Q + k * 8, desc_k_major(ka + (i & 1) * S::STAGE + (k >> 2) * S::KCH + (k & 3) * 32), S::IDESC_S,
-                           k > 0 ? 1u : 0u);
-                mma_commit(&sh.s_full[i & 1]);
+                for (int k = 0; k < D / 16; k++) mma_ts(d, tm + S::COL_Q + k * 8, desc + (((k >> 2) * S::KCH + (k & 3) * 32) >> 4), S::IDESC_S, k > 0 ? 1u : 0u, leader);
+                mma_commit_by(&sh.s_full[i & 1], leader);
             };
-            wait(&sh.q_full, 0);
+            all_wait(&sh.q_full, 0);
             scores(0);
             for (uint32_t i = 0; i < nt && ok; i++) {
                 if (i + 1 < nt) scores(i + 1);
-                wait(&sh.p_ready[i & 1], (i >> 1) & 1);
-                wait(&sh.v_full[i & 1], (i >> 1) & 1);
+                all_wait(&sh.p_ready[i & 1], (i >> 1) & 1);
+                all_wait(&sh.v_full[i & 1], (i >> 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t desc = v_desc + (i & 1) * (S::STAGE >> 4);
+                const uint32_t p = tm + S::COL_S + (i & 1) * KT;
 #pragma unroll
-                for (int k = 0; k < KT / 16; k++)
-                    mma_ts(tmem + S::COL_O, tmem + S::COL_S + (i & 1) * KT + k * 8, desc_mn_major(va + (i & 1) * S::STAGE + k * 2048, S::KCH), S::IDESC_PV,
-                           (i > 0 || k > 0) ? 1u : 0u);
-                mma_commit(&sh.pv_done[i % AHEAD]);
+                for (int k = 0; k < KT / 16; k++) mma_ts(tm + S::COL_O, p + k * 8, desc + (k * 2048 >> 4), S::IDESC_PV, k > 0 ? 1u : i > 0 ? 1u : 0u, leader);
+                mma_commit_by(&sh.pv_done[i % AHEAD], leader);
             }
             if (!ok) {  // a wait ran out: nothing may still write tensor memory when it is given back
-                mma_commit(&sh.drained);
+                mma_commit_by(&sh.drained, leader);
                 mbar_wait(&sh.drained, 0);
             }
         }
         __syncwarp();
     } else {
         // ---- the tiles ahead -------------------------------------------------------------------------------------------
-        const uint32_t page = 1u << a.shift, count = page < (uint32_t)KT ? KT / page : 1;
+        // A lane a page, as many tiles at once as 32 lanes have pages for; page numbers are asked for two such batches ahead, scales one:
+        // looked up tile by tile, the two trips to the L2 behind one another took longer than everything else about a tile.
+        const uint32_t page = 1u << a.shift, count = page < (uint32_t)KT ? KT / page : 1, tiles = 32 / count;
+        auto page_at = [&](uint32_t b) {  // this lane's page of the batch of tiles that starts with tile b
+            const uint32_t j = tile0 + (b + lane / count) * KT + lane % count * page;
+            const uint32_t id = (j & ~(page - 1)) < end ? __ldg(a.table + (size_t)r * a.width + (j >> a.shift)) : 0xffffffffu;
+            return id < a.pages ? id : 0xffffffffu;
+        };
+        auto scales_at = [&](uint32_t id) {
+            const size_t at = (size_t)id * a.kv_heads + kvh;
+            return id != 0xffffffffu ? make_float2(__ldg(a.ks + at), __ldg(a.vs + at)) : make_float2(0.0f, 0.0f);
+        };
+        auto pair = [](float f) {
+            const __half2 h = __float2half2_rn(f), o = __hmul2(h, __half2half2(__ushort_as_half(0xe480)));  // -1152
+            return make_uint2(*reinterpret_cast<const uint32_t*>(&h), *reinterpret_cast<const uint32_t*>(&o));
+        };
+        uint32_t id = 0xffffffffu, id1 = 0xffffffffu;
+        float2 sc = make_float2(0.0f, 0.0f);
+        if (nt != 0) id = page_at(0), id1 = page_at(tiles), sc = scales_at(id);
         float vref = 0.0f;
-        for (uint32_t i = 0; i < nt; i++) {
-            if (i >= AHEAD) wait(&sh.pv_done[i % AHEAD], (i / AHEAD - 1) & 1);  // nobody reads the entry's old tile any more
-            const uint32_t j0 = tile0 + i * KT, j = j0 + lane * page;
-            uint32_t id = 0xffffffffu;
-            if (lane < count && (j & ~(page - 1)) < end) id = __ldg(a.table + (size_t)r * a.width + (j >> a.shift));
-            if (id >= a.pages) id = 0xffffffffu;
-            float ks = 0.0f, vs = 0.0f;
-            if (id != 0xffffffffu) ks = __ldg(a.ks + (size_t)id * a.kv_heads + kvh), vs = __ldg(a.vs + (size_t)id * a.kv_heads + kvh);
-            const float kref = warp_max(ks), vnew = fmaxf(vref, warp_max(vs));
-            Ahead& info = sh.ahead[i % AHEAD];
-            if (lane < MOST_PAGES) {
-                info.id[lane] = id;
-                const __half2 kf = __float2half2_rn(kref > 0.0f ? __fdiv_rn(ks, kref) : 0.0f), vf = __float2half2_rn(vnew > 0.0f ? __fdiv_rn(vs, vnew) : 0.0f);
-                info.kf[lane] = *reinterpret_cast<const uint32_t*>(&kf), info.vf[lane] = *reinterpret_cast<const uint32_t*>(&vf);
-            }
+        for (uint32_t b = 0; b < nt; b += tiles) {
+            const float2 sc1 = scales_at(id1);
+            const uint32_t id2 = page_at(b + 2 * tiles);
             const uint32_t has = __ballot_sync(0xffffffffu, id != 0xffffffffu);
-            if (lane < 4) {
-                uint32_t keys = 0;
-                for (uint32_t e = 0; e < 32; e++) {
-                    const uint32_t c = lane * 32 + e, pg = page < (uint32_t)KT ? c >> a.shift : 0;
-                    if (c < (uint32_t)KT && ((has >> pg) & 1u)) keys |= 1u << e;
+            float km = sc.x, vm = sc.y;  // the tile's largest
+            for (uint32_t o = 1; o < count; o <<= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o)), vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+            const uint2 kf = pair(km > 0.0f ? __fdiv_rn(sc.x, km) : 0.0f);
+            for (uint32_t t = 0; t < tiles && b + t < nt; t++) {
+                const uint32_t i = b + t, j0 = tile0 + i * KT;
+                const float vnew = fmaxf(vref, __shfl_sync(0xffffffffu, vm, t * count));
+                if (i >= AHEAD) wait(&sh.pv_done[i % AHEAD], (i / AHEAD - 1) & 1);  // nobody reads the entry's old tile any more
+                Ahead& info = sh.ahead[i % AHEAD];
+                if (lane / count == t) {
+                    const uint32_t k = lane % count;
+                    info.at[k] = ((((unsigned long long)(id != 0xffffffffu ? id : 0) * a.kv_heads + kvh) << a.shift) + (page > (uint32_t)KT ? j0 & (page - 1) : 0)) * D;
+                    info.kf[k] = kf, info.vf[k] = pair(vnew > 0.0f ? __fdiv_rn(sc.y, vnew) : 0.0f);
+                    if (k == 0) {
+                        info.kref = km, info.shrink = vref > 0.0f ? __fdiv_rn(vref, vnew) : 1.0f;
+                        if (i + 1 == nt) sh.vref = vnew;
+                    }
                 }
-                info.keys[lane] = keys;
+                if (lane < KT / 32) {
+                    uint32_t keys = 0;
+                    const uint32_t mine = has >> (t * count);
+                    if (page >= (uint32_t)KT) keys = mine & 1u ? 0xffffffffu : 0u;
+                    else if (page >= 32) keys = (mine >> (lane * 32 >> a.shift)) & 1u ? 0xffffffffu : 0u;
+                    else keys = ((mine >> (2 * lane)) & 1u ? 0xffffu : 0u) | ((mine >> (2 * lane + 1)) & 1u ? 0xffff0000u : 0u);  // pages of 16
+                    info.keys[lane] = keys;
+                }
+                vref = vnew;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.known[i % AHEAD]);
             }
-            if (lane == 0) {
-                info.kref = kref;
-                info.shrink = vref > 0.0f ? __fdiv_rn(vref, vnew) : 1.0f;
-                if (i + 1 == nt) sh.vref = vnew;
-            }
-            vref = vnew;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.known[i % AHEAD]);
+            id = id1, id1 = id2, sc = sc1;
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 template <int D>
