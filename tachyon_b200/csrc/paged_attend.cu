@@ -4,13 +4,15 @@
 // number, and that is what bounds it.  The work of all requests is laid out in a line of tiles of 64 positions (request, then
 // key-value head, then tile) and cut into equal shares, one a block, whatever the lengths: a prefix sum over the requests, repeated
 // by every block, finds a block's place.  A block whose share ends inside a line of keys leaves its maximum, sum and outputs in
-// scratch, and the last of that line's blocks to arrive (a counter, nobody waits) adds them up in the order of the positions.
+// scratch; the last of 32 neighbours to arrive (a counter, nobody waits) adds theirs up, the last of the line's sets of 32 adds up
+// those, always in the order of the positions.
 //
-// A warp takes 16 positions at a time straight from global memory into the operands of mma.sync.m16n8k16; tcgen05 has no place
-// here, a tile of 64 keys against 8 query rows is two orders of magnitude below one of its tiles.  A sum does not mind the order
-// of its terms, so the operands' order is chosen for the loads: a thread's four dimensions (or tokens) of an MMA step lie side by
-// side in memory, and 16 bytes of a row feed four steps.  A code becomes f16 by byte permutes: 0x6400 | (code + 128) is
-// 1152 + code, one packed subtraction leaves the code, exactly.
+// A warp takes 16 positions at a time.  It copies their codes into a ring of its own in shared memory (cp.async, a few slices ahead, so
+// that no barrier is needed and no register holds what is on its way) and reads them from there as operands of mma.sync.m16n8k16;
+// tcgen05 has no place here, a tile of 64 keys against 8 query rows is two orders of magnitude below one of its tiles.  A sum does
+// not mind the order of its terms, so the operands' order is chosen for the loads: a thread's four dimensions (or tokens) of an MMA
+// step lie side by side, 16 bytes of a row feed four steps, and the 16-byte pieces of a row are permuted so that eight lanes meet no
+// bank twice.  A code becomes f16 by byte permutes: 0x6400 | (code + 128) is 1152 + code, one packed subtraction leaves the code.
 //   S = Q K^T: rows 0-7 of the A operand hold the queries rounded to f16, rows 8-15 what the rounding left, so the sum of the
 //   two halves is the f32 product to 2^-22; the page's scale, a power of two, multiplies the score.
 //   O^T = V^T P^T: the scores' accumulator is the B operand's layout as it stands; the weights again go in two f16 parts.  A page's
@@ -23,8 +25,22 @@ namespace tb {
 
 namespace {
 
-constexpr uint32_t TILE = 64, SLICE = 16;
-constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr uint32_t TILE = 64;
+constexpr uint32_t CHUNKS = MAX_REQUESTS / 32;  // chunks of 32 requests, a lane each, with a prefix sum over them
+constexpr uint32_t SET = 32;          // partial results of a line that one block adds up
+
+template <int D>
+struct Shape {
+    // Warps as registers allow (D / 4 hold the output), rings as shared memory does: 16 to 32 KiB a warp, a slice in use and the others
+    // on their way.
+    static constexpr int WARPS = D == 512 ? 6 : 4, THREADS = WARPS * 32, RESIDENT = D == 512 ? 1 : 3;  // blocks a multiprocessor
+    static constexpr int SLICE = D <= 128 ? 32 : 16, HALVES = SLICE / 16;  // positions a warp takes at a time; a page holds sixteen at least
+    static constexpr int STAGES = D == 64 ? 4 : 2;
+    static constexpr int HALF = 16 * D, STAGE = 2 * HALVES * HALF;  // sixteen positions' keys (or values); a slice's keys, then its values
+    static constexpr int OFF_RING = D * 32, RING = STAGES * STAGE, BYTES = OFF_RING + WARPS * RING;
+    static_assert(RING >= 8 * D * 4, "a warp's outputs go over its ring at the end of a line");
+    static_assert(RESIDENT * (BYTES + 4096) <= 228 * 1024, "over what a multiprocessor has");
+};
 
 struct PagedArgs {
     const int8_t* k;
@@ -37,9 +53,9 @@ struct PagedArgs {
     const uint32_t* lengths;
     void* out;
     float* partial;           // [2 * blocks][16 + 8 * D]
-    uint32_t* count;          // [blocks]: of the line that the block begins and does not finish
+    uint32_t* count;          // [512]: of the line that a block begins and does not finish; [512]: of the set that a block is first of
     unsigned long long q_stride, out_stride;
-    uint32_t pages, shift, kv_heads, requests, width, tokens, heads, ratio, most, window, least;
+    uint32_t pages, shift, kv_heads, requests, width, tokens, heads, ratio, most, window;
     float scale;              // softmax scale times log2(e)
     int q_f16, out_f16;
 };
@@ -50,7 +66,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -65,15 +81,23 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 load_stream2(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Where 16-byte piece c of row r of a slice lies.  Keys are read by eight lanes as four pieces of two neighbouring rows, values as two
+// pieces of rows 0, 2, 4, 6 (or 1, 3, 5, 7): no bank twice in either.
+template <int D>
+__device__ __forceinline__ uint32_t key_at(uint32_t r, uint32_t c) {
+    return D == 64 ? r * 64 + c * 16 : r * D + ((c ^ ((r & 1) << 2)) << 4);
+}
+template <int D>
+__device__ __forceinline__ uint32_t value_at(uint32_t r, uint32_t c) {
+    return D == 64 ? (r >> 1) * 128 + (((r & 1) ^ ((r >> 2) & 1)) << 6) + ((c ^ (r & 2)) << 4) : r * D + ((c ^ (r & 6)) << 4);
 }
 
 // What a request asks for, from device memory that may hold anything: clamped so that nothing out of range is touched.
@@ -97,94 +121,165 @@ __device__ __forceinline__ Request request_of(const PagedArgs& a, uint32_t r) {
 }
 
 template <int D>
-constexpr size_t smem_bytes() {
-    return (size_t)D * 32 + WARPS * 8 * (size_t)D * 4 + WARPS * 16 * 4 + 64;
-}
-
-template <int D>
-__global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) paged_attend_kernel(const PagedArgs a) {
-    constexpr int MT = D / 16, SEG = D / 64;
-    extern __shared__ __align__(16) uint8_t raw[];
+__global__ void __launch_bounds__(Shape<D>::THREADS, Shape<D>::RESIDENT) paged_attend_kernel(const PagedArgs a) {
+    using S = Shape<D>;
+    constexpr int MT = D / 16, SEG = D / 64, WARPS = S::WARPS, THREADS = S::THREADS, STAGES = S::STAGES, SLICE = S::SLICE, HALVES = S::HALVES;
+    extern __shared__ __align__(128) uint8_t raw[];
     uint4* s_q = reinterpret_cast<uint4*>(raw);                      // [D / 16][32]: the A operand of every step
-    float* s_acc = reinterpret_cast<float*>(raw + D * 32);           // [WARPS][8][D]
-    float* s_m = s_acc + WARPS * 8 * D;                              // [WARPS][8]
-    float* s_l = s_m + WARPS * 8;
-    float* s_row = s_l + WARPS * 8;                                  // [8]: a query row's factor
-    uint32_t* s_flag = reinterpret_cast<uint32_t*>(s_row + 8);
-    uint32_t* s_sum = s_flag + 8;                                    // [requests + 1]: tiles before each request
-    __shared__ uint32_t part[WARPS];
+    __shared__ float s_m[WARPS * 8], s_l[WARPS * 8];
+    __shared__ uint32_t s_chunk[CHUNKS + 1];
+    __shared__ float s_row[8], s_wt[2][8];
+    __shared__ uint32_t s_flag;
     const uint32_t th = threadIdx.x, lane = th & 31, warp = th >> 5, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = raw + S::OFF_RING + warp * S::RING;
     pdl_wait();
 
-    {  // tiles before each request
-        const uint32_t per = (a.requests + THREADS - 1) / THREADS, r0 = min(th * per, a.requests), r1 = min(r0 + per, a.requests);
-        uint32_t mine = 0;
-        for (uint32_t r = r0; r < r1; r++) {
-            const Request q = request_of(a, r);
-            mine += q.tiles * q.groups * a.kv_heads;
-        }
-        uint32_t x = mine;
+    // Tiles before each request: a lane a request of one chunk of 32 (`rq`, and `sum` up to and with it).  With more than one chunk the
+    // block first adds up all of them.
+    Request mine;
+    uint32_t chunk = 0, sum;
+    auto look = [&](uint32_t c) {
+        const uint32_t r = c * 32 + lane;
+        mine.tiles = mine.groups = mine.n = 0;
+        if (r < a.requests) mine = request_of(a, r);
+        uint32_t x = mine.tiles * mine.groups * a.kv_heads;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= (uint32_t)o) x += y;
         }
-        if (lane == 31) part[warp] = x;
-        __syncthreads();
-        uint32_t at = x - mine;
-        for (uint32_t w = 0; w < warp; w++) at += part[w];
-        for (uint32_t r = r0; r < r1; r++) {
-            const Request q = request_of(a, r);
-            s_sum[r] = at;
-            at += q.tiles * q.groups * a.kv_heads;
-            if (r + 1 == a.requests) s_sum[a.requests] = at;
+        return x;
+    };
+    uint32_t total;
+    if (a.requests <= 32) {
+        sum = look(0);
+        total = __shfl_sync(0xffffffffu, sum, 31);
+    } else {
+        const uint32_t chunks = (a.requests + 31) / 32;
+        for (uint32_t c = warp; c < chunks; c += WARPS) {
+            const uint32_t x = look(c);
+            if (lane == 31) s_chunk[c] = x;
         }
         __syncthreads();
+        if (warp == 0) {
+            uint32_t x = 0, v[CHUNKS / 32];
+#pragma unroll
+            for (uint32_t e = 0; e < CHUNKS / 32; e++) v[e] = x, x += lane * (CHUNKS / 32) + e < chunks ? s_chunk[lane * (CHUNKS / 32) + e] : 0;
+            uint32_t y = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= (uint32_t)o) y += z;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < CHUNKS / 32; e++) s_chunk[lane * (CHUNKS / 32) + e] = y - x + v[e];
+            if (lane == 31) s_chunk[CHUNKS] = y;
+        }
+        __syncthreads();
+        total = s_chunk[CHUNKS];
+        chunk = 0xffffffffu;
     }
-    const uint32_t total = s_sum[a.requests];
     if (total == 0) return;
-    const uint32_t blocks = min(gridDim.x, (total + a.least - 1) / a.least);
+    // Equal shares, the first `more` of them a tile larger; the block that has a tile.
+    // Two tiles a block at least once there are enough for every other block of a small launch: halves what has to be added up again.
+    const uint32_t blocks = min(gridDim.x, total <= 64 ? total : (total + 1) / 2);
     if (blockIdx.x >= blocks) return;
-    const uint32_t my0 = (uint32_t)((unsigned long long)total * blockIdx.x / blocks), my1 = (uint32_t)((unsigned long long)total * (blockIdx.x + 1) / blocks);
+    const uint32_t share = total / blocks, more = total - share * blocks;
+    const uint32_t my0 = share * blockIdx.x + min(blockIdx.x, more), my1 = my0 + share + (blockIdx.x < more ? 1 : 0);
+    auto block_of = [&](uint32_t x) { return x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share; };
 
     for (uint32_t at = my0; at < my1;) {
-        uint32_t lo = 0, hi = a.requests;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (s_sum[mid] <= at) lo = mid;
-            else hi = mid;
+        // The request that tile `at` belongs to: its chunk by bisection (the last one that starts at or before it), then by lane.
+        uint32_t offset = 0;
+        if (a.requests > 32) {
+            uint32_t lo = 0, hi = (a.requests + 31) / 32;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (s_chunk[mid] <= at) lo = mid;
+                else hi = mid;
+            }
+            if (lo != chunk) sum = look(lo);
+            chunk = lo;
+            offset = s_chunk[lo];
         }
-        // Requests without tiles share their successor's place: `lo` is the last with that sum, the one that has tiles.
-        const uint32_t r = lo;
-        const Request rq = request_of(a, r);
-        const uint32_t line = (at - s_sum[r]) / rq.tiles, tile0 = (at - s_sum[r]) % rq.tiles;
+        const uint32_t here = mine.tiles * mine.groups * a.kv_heads;
+        const uint32_t who = __ffs(__ballot_sync(0xffffffffu, here != 0 && at < offset + sum)) - 1;
+        const uint32_t r = chunk * 32 + who, before = __shfl_sync(0xffffffffu, offset + sum - here, who);
+        Request rq;
+        rq.first = __shfl_sync(0xffffffffu, mine.first, who), rq.n = __shfl_sync(0xffffffffu, mine.n, who), rq.len = __shfl_sync(0xffffffffu, mine.len, who);
+        rq.low = __shfl_sync(0xffffffffu, mine.low, who), rq.tiles = __shfl_sync(0xffffffffu, mine.tiles, who), rq.groups = __shfl_sync(0xffffffffu, mine.groups, who);
+        const uint32_t line = (at - before) / rq.tiles, tile0 = (at - before) % rq.tiles;
         const uint32_t kvh = line / rq.groups, group = line % rq.groups;
-        const uint32_t line0 = s_sum[r] + line * rq.tiles;  // the line's first tile
+        const uint32_t line0 = before + line * rq.tiles;  // the line's first tile
         const uint32_t tile1 = min(rq.tiles, tile0 + (my1 - at));
         at += tile1 - tile0;
 
-        // The queries of this line: row i is (token i / ratio, head i % ratio) of the group's eight, scaled so that its largest
-        // lies in [1, 2), in two f16 parts, in the order the MMA wants them.
-        {
-            const uint32_t row = group * 8 + warp, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
-            const bool real = tok < rq.n;
-            float x[D / 32];
+        // This warp's slices: positions start + SLICE WARPS i on, up to `end`.  A lane looks up the page of the sixteen positions with its
+        // number (mod 32), for this batch of 32 and the next.
+        const uint32_t start = rq.low + tile0 * TILE + warp * SLICE, end = min(rq.len, rq.low + tile1 * TILE);
+        const uint32_t slices = start < end ? (end - start + WARPS * SLICE - 1) / (WARPS * SLICE) : 0;
+        auto page_at = [&](uint32_t x) {
+            const uint32_t j = start + x / HALVES * (WARPS * SLICE) + x % HALVES * 16;
+            const uint32_t id = j < end ? __ldg(a.table + (size_t)r * a.width + (j >> a.shift)) : 0xffffffffu;
+            return id < a.pages ? id : 0xffffffffu;
+        };
+        auto scales_at = [&](uint32_t id) {
+            const size_t p = (size_t)id * a.kv_heads + kvh;
+            return id != 0xffffffffu ? make_float2(__ldg(a.ks + p), __ldg(a.vs + p)) : make_float2(0.0f, 0.0f);
+        };
+        uint32_t id = page_at(lane), id1 = page_at(32 + lane);
+        // The queries of this line, asked for before anything waits for the pages: row i is (token i / ratio, head i % ratio) of the
+        // group's eight, scaled so that its largest lies in [1, 2), in two f16 parts, in the order the MMA wants them.
+        constexpr uint32_t QROWS = (8 + WARPS - 1) / WARPS;
+        float qx[QROWS][D / 32];
+#pragma unroll
+        for (uint32_t k = 0; k < QROWS; k++) {
+            const uint32_t row = group * 8 + warp + k * WARPS, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
+            const unsigned long long p = (unsigned long long)(rq.first + tok) * a.q_stride + (unsigned long long)head * D + lane;
+#pragma unroll
+            for (int e = 0; e < D / 32; e++)
+                qx[k][e] = tok >= rq.n || warp + k * WARPS >= 8 ? 0.0f : a.q_f16 ? __half2float(static_cast<const __half*>(a.q)[p + e * 32]) : static_cast<const float*>(a.q)[p + e * 32];
+        }
+        float2 sc = scales_at(id), sc1 = make_float2(0.0f, 0.0f);
+        const uint32_t inside = (1u << a.shift) - 1;
+        uint32_t to = 0;  // the stage that is filled next
+        auto fetch = [&](uint32_t i, uint32_t base) {  // slice i into its stage; base: the first sixteen of the batch that `id` is of
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) {
+                const uint32_t x = i * HALVES + h, pid = __shfl_sync(0xffffffffu, x < base + 32 ? id : id1, x & 31);
+                if (i < slices && pid != 0xffffffffu) {
+                    const uint32_t j = start + i * (WARPS * SLICE) + h * 16;
+                    const size_t from = ((((size_t)pid * a.kv_heads + kvh) << a.shift) + (j & inside)) * D + lane * 16;
+                    uint8_t* stage = ring + to * S::STAGE + h * S::HALF;
+#pragma unroll
+                    for (int e = 0; e < D / 32; e++) copy16(stage + key_at<D>((e * 32 + lane) / (D / 16), (e * 32 + lane) % (D / 16)), a.k + from + e * 512);
+#pragma unroll
+                    for (int e = 0; e < D / 32; e++)
+                        copy16(stage + HALVES * S::HALF + value_at<D>((e * 32 + lane) / (D / 16), (e * 32 + lane) % (D / 16)), a.v + from + e * 512);
+                }
+            }
+            copy_commit();
+            to = to + 1 == STAGES ? 0 : to + 1;
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) fetch(i, 0);
+
+#pragma unroll
+        for (uint32_t k = 0; k < QROWS; k++) {
+            const uint32_t mine_row = warp + k * WARPS;
+            if (mine_row >= 8) break;
             float big = 0.0f;
 #pragma unroll
-            for (int e = 0; e < D / 32; e++) {
-                const unsigned long long p = (unsigned long long)(rq.first + tok) * a.q_stride + (unsigned long long)head * D + e * 32 + lane;
-                x[e] = !real ? 0.0f : a.q_f16 ? __half2float(static_cast<const __half*>(a.q)[p]) : static_cast<const float*>(a.q)[p];
-                big = fmaxf(big, fabsf(x[e]));
-            }
+            for (int e = 0; e < D / 32; e++) big = fmaxf(big, fabsf(qx[k][e]));
             big = warp_max(big);
             const uint32_t expo = min(max(__float_as_uint(big) >> 23, 1u), 253u);  // infinities stay what they are
             const float inv = __uint_as_float((254u - expo) << 23);
-            if (lane == 0) s_row[warp] = a.scale * __uint_as_float(expo << 23);
+            if (lane == 0) s_row[mine_row] = a.scale * __uint_as_float(expo << 23);
             __half* dst = reinterpret_cast<__half*>(s_q);
 #pragma unroll
             for (int e = 0; e < D / 32; e++) {
-                const uint32_t d = e * 32 + lane, step = d / 64 * 4 + d % 16 / 4, owner = warp * 4 + d % 64 / 16, reg = (d & 2), half = d & 1;
-                const float y = x[e] * inv;
+                const uint32_t d = e * 32 + lane, step = d / 64 * 4 + d % 16 / 4, owner = mine_row * 4 + d % 64 / 16, reg = (d & 2), half = d & 1;
+                const float y = qx[k][e] * inv;
                 const __half h = __float2half_rn(y);
                 __half* p = dst + ((step * 32 + owner) * 4 + reg) * 2 + half;
                 p[0] = h;
@@ -201,103 +296,133 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) paged_attend_kernel
         const int pos = my_tok < rq.n ? (int)rq.len - (int)rq.n + (int)my_tok : -1;  // negative: this row sees nothing
         const int oldest = a.window != 0 && pos >= (int)a.window ? pos + 1 - (int)a.window : 0;
         const float factor = s_row[g];
-        const uint32_t end = min(rq.len, rq.low + tile1 * TILE);
-        for (uint32_t j0 = rq.low + tile0 * TILE + warp * SLICE; j0 < end; j0 += WARPS * SLICE) {
-            const uint32_t id = __ldg(a.table + (size_t)r * a.width + (j0 >> a.shift));
-            if (id >= a.pages) continue;  // no page: nothing to see
-            const size_t ph = (size_t)id * a.kv_heads + kvh;
-            const size_t row0 = (ph << a.shift) + (j0 & ((1u << a.shift) - 1));
-            const int8_t* kp = a.k + row0 * D;
-            const int8_t* vp = a.v + row0 * D;
-            const float ks = __ldg(a.ks + ph) * factor, vs = __ldg(a.vs + ph);
-            // Scores of tokens j0 + 2t, + 1 (c[0]) and j0 + 8 + 2t, + 1 (c[1]) for query row g.
-            float c[2][4] = {};
-            uint4 kw[2][SEG];
+        uint32_t at_stage = 0;
+        for (uint32_t i = 0; i < slices; i++) {
+            const uint32_t x0 = i * HALVES, base = x0 & ~31u;
+            if (i != 0 && x0 == base) id = id1, sc = sc1, id1 = page_at(base + 32 + lane);
+            if ((x0 & 31) == 16) sc1 = scales_at(id1);
+            copy_wait<STAGES - 2>();
+            __syncwarp();  // every lane's copies of this slice are there, and every lane is done with the stage that is filled next
+            fetch(i + STAGES - 1, base);
+            float ks[HALVES], vs[HALVES];
+            bool real[HALVES];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int s = 0; s < SEG; s++) kw[j][s] = load_stream(kp + (j * 8 + g) * D + s * 64 + t * 16);
+            for (int h = 0; h < HALVES; h++) {
+                real[h] = __shfl_sync(0xffffffffu, id, (x0 + h) & 31) != 0xffffffffu;  // no page: nothing to see
+                ks[h] = __shfl_sync(0xffffffffu, sc.x, (x0 + h) & 31) * factor, vs[h] = __shfl_sync(0xffffffffu, sc.y, (x0 + h) & 31);
+            }
+            const uint32_t j0 = start + i * (WARPS * SLICE);
+            const uint8_t* kp = ring + at_stage * S::STAGE;
+            const uint8_t* vp = kp + HALVES * S::HALF;
+            at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
+            // Scores of tokens 8 j + 2 t, + 1 of the slice (c[j]) for query row g.
+            // Four accumulators at least, so that the products need not wait for one another.
+            constexpr int SPLIT = HALVES == 1 ? 2 : 1;
+            float c[2 * HALVES * SPLIT][4] = {};
 #pragma unroll
             for (int s = 0; s < SEG; s++) {
+                uint4 k[2 * HALVES];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint4 q = s_q[(s * 4 + i) * 32 + lane];
+                for (int j = 0; j < 2 * HALVES; j++) k[j] = *reinterpret_cast<const uint4*>(kp + (j >> 1) * S::HALF + key_at<D>((j & 1) * 8 + g, s * 4 + t));
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t w = (i == 0 ? kw[j][s].x : i == 1 ? kw[j][s].y : i == 2 ? kw[j][s].z : kw[j][s].w) ^ 0x80808080u;
-                        mma16816(c[j], q.x, q.y, q.z, q.w, halves(w, LOW), halves(w, HIGH));
+                for (int e = 0; e < 4; e++) {
+                    const uint4 q = s_q[(s * 4 + e) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < 2 * HALVES; j++) {
+                        const uint32_t w = (e == 0 ? k[j].x : e == 1 ? k[j].y : e == 2 ? k[j].z : k[j].w) ^ 0x80808080u;
+                        mma16816(c[j + (e & (SPLIT - 1)) * 2 * HALVES], q.x, q.y, q.z, q.w, halves(w, LOW), halves(w, HIGH));
                     }
                 }
             }
-            float s[4] = {(c[0][0] + c[0][2]) * ks, (c[0][1] + c[0][3]) * ks, (c[1][0] + c[1][2]) * ks, (c[1][1] + c[1][3]) * ks};
+            if constexpr (SPLIT == 2)
+#pragma unroll
+                for (int j = 0; j < 2 * HALVES; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[j][e] += c[j + 2 * HALVES][e];
+            float s[2 * HALVES][2];
             float top = m;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = (int)j0 + (e >> 1) * 8 + 2 * (int)t + (e & 1);
-                if (j > pos || j < oldest) s[e] = -INFINITY;
-                top = fmaxf(top, s[e]);
-            }
+            for (int j = 0; j < 2 * HALVES; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int at_j = (int)j0 + j * 8 + 2 * (int)t + e;
+                    s[j][e] = at_j > pos || at_j < oldest || !real[j >> 1] ? -INFINITY : (c[j][e] + c[j][2 + e]) * ks[j >> 1];
+                    top = fmaxf(top, s[j][e]);
+                }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float base = top == -INFINITY ? 0.0f : top;
-            const float corr = ex2(m - base);  // 0 before the first visible key
+            const float from = top == -INFINITY ? 0.0f : top;
+            float turn = ex2(m - from);  // 0 before the first visible key
             m = top;
-            const float vnew = fmaxf(vref, vs);
-            const float ratio = vnew > 0.0f ? __fdiv_rn(vs, vnew) : 0.0f, shrink = vnew > 0.0f ? __fdiv_rn(vref, vnew) : 0.0f;
-            vref = vnew;
-            float w[4];
-            float sum = 0.0f;
+            float ratio[HALVES];
+            float vnew = vref;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p = ex2(s[e] - base);
-                sum += p;
-                w[e] = p * ratio;
+            for (int h = 0; h < HALVES; h++) ratio[h] = 1.0f, vnew = fmaxf(vnew, vs[h]);
+            const float corr = turn;
+            if (vnew != vref || vs[0] != vref || vs[HALVES - 1] != vref) {  // the same in every lane
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) ratio[h] = vnew > 0.0f ? __fdiv_rn(vs[h], vnew) : 0.0f;
+                turn *= vnew > 0.0f ? __fdiv_rn(vref, vnew) : 0.0f;
+                vref = vnew;
+            }
+            float sum = 0.0f;
+            uint32_t hi[2 * HALVES], lo[2 * HALVES];
+#pragma unroll
+            for (int j = 0; j < 2 * HALVES; j++) {
+                const float p0 = ex2(s[j][0] - from), p1 = ex2(s[j][1] - from);
+                sum += p0 + p1;
+                const float w0 = p0 * ratio[j >> 1], w1 = p1 * ratio[j >> 1];
+                hi[j] = pack(w0, w1);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
+                lo[j] = pack(w0 - f.x, w1 - f.y);
             }
             l = fmaf(l, corr, sum);
-            const float turn = corr * shrink;
             if (__any_sync(0xffffffffu, turn != 1.0f)) {
                 const float c0 = __shfl_sync(0xffffffffu, turn, 8 * t), c1 = __shfl_sync(0xffffffffu, turn, 8 * t + 4);  // rows 2t, 2t + 1
 #pragma unroll
-                for (int i = 0; i < MT; i++) acc[i][0] *= c0, acc[i][1] *= c1, acc[i][2] *= c0, acc[i][3] *= c1;
+                for (int k = 0; k < MT; k++) acc[k][0] *= c0, acc[k][1] *= c1, acc[k][2] *= c0, acc[k][3] *= c1;
             }
-            const uint32_t h0 = pack(w[0], w[1]), h1 = pack(w[2], w[3]);
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-            const uint32_t l0 = pack(w[0] - f0.x, w[1] - f0.y), l1 = pack(w[2] - f1.x, w[3] - f1.y);
-            // Values of tokens 2t, 2t + 1, 2t + 8, 2t + 9; four dimensions of the four tokens make two MMA tiles' A operands.
-            auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, float (&even)[4], float (&odd)[4]) {
-                wa ^= 0x80808080u, wb ^= 0x80808080u, wc ^= 0x80808080u, wd ^= 0x80808080u;
-                const uint32_t ab = __byte_perm(wa, wb, 0x5140), cd = __byte_perm(wc, wd, 0x5140), ab2 = __byte_perm(wa, wb, 0x7362), cd2 = __byte_perm(wc, wd, 0x7362);
-                const uint32_t e0 = halves(ab, LOW), e1 = halves(ab, HIGH), e2 = halves(cd, LOW), e3 = halves(cd, HIGH);
-                mma16816(even, e0, e1, e2, e3, h0, h1);
-                mma16816(even, e0, e1, e2, e3, l0, l1);
-                const uint32_t o0 = halves(ab2, LOW), o1 = halves(ab2, HIGH), o2 = halves(cd2, LOW), o3 = halves(cd2, HIGH);
-                mma16816(odd, o0, o1, o2, o3, h0, h1);
-                mma16816(odd, o0, o1, o2, o3, l0, l1);
-            };
-            if constexpr (D == 64) {
-                const uint2 va = load_stream2(vp + (2 * t) * D + g * 8), vb = load_stream2(vp + (2 * t + 1) * D + g * 8);
-                const uint2 vc = load_stream2(vp + (2 * t + 8) * D + g * 8), vd = load_stream2(vp + (2 * t + 9) * D + g * 8);
-                four(va.x, vb.x, vc.x, vd.x, acc[0], acc[1]);
-                four(va.y, vb.y, vc.y, vd.y, acc[2], acc[3]);
-            } else {
 #pragma unroll
-                for (int sg = 0; sg < D / 128; sg++) {
-                    const int8_t* p = vp + sg * 128 + g * 16;
-                    const uint4 va = load_stream(p + (2 * t) * D), vb = load_stream(p + (2 * t + 1) * D), vc = load_stream(p + (2 * t + 8) * D),
-                                vd = load_stream(p + (2 * t + 9) * D);
-                    four(va.x, vb.x, vc.x, vd.x, acc[sg * 8], acc[sg * 8 + 1]);
-                    four(va.y, vb.y, vc.y, vd.y, acc[sg * 8 + 2], acc[sg * 8 + 3]);
-                    four(va.z, vb.z, vc.z, vd.z, acc[sg * 8 + 4], acc[sg * 8 + 5]);
-                    four(va.w, vb.w, vc.w, vd.w, acc[sg * 8 + 6], acc[sg * 8 + 7]);
+            for (int h = 0; h < HALVES; h++) {
+                const uint8_t* v = vp + h * S::HALF;
+                const uint32_t h0 = hi[2 * h], h1 = hi[2 * h + 1], l0 = lo[2 * h], l1 = lo[2 * h + 1];
+                // Values of tokens 2t, 2t + 1, 2t + 8, 2t + 9; four dimensions of the four tokens make two MMA tiles' A operands.
+                auto four = [&](uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd, float (&even)[4], float (&odd)[4]) {
+                    const uint32_t ab = __byte_perm(wa, wb, 0x5140) ^ 0x80808080u, cd = __byte_perm(wc, wd, 0x5140) ^ 0x80808080u;
+                    const uint32_t ab2 = __byte_perm(wa, wb, 0x7362) ^ 0x80808080u, cd2 = __byte_perm(wc, wd, 0x7362) ^ 0x80808080u;
+                    const uint32_t e0 = halves(ab, LOW), e1 = halves(ab, HIGH), e2 = halves(cd, LOW), e3 = halves(cd, HIGH);
+                    mma16816(even, e0, e1, e2, e3, h0, h1);
+                    const uint32_t o0 = halves(ab2, LOW), o1 = halves(ab2, HIGH), o2 = halves(cd2, LOW), o3 = halves(cd2, HIGH);
+                    mma16816(odd, o0, o1, o2, o3, h0, h1);
+                    mma16816(even, e0, e1, e2, e3, l0, l1);
+                    mma16816(odd, o0, o1, o2, o3, l0, l1);
+                };
+                if constexpr (D == 64) {
+                    auto row = [&](uint32_t r2) { return *reinterpret_cast<const uint2*>(v + value_at<D>(r2, g >> 1) + (g & 1) * 8); };
+                    const uint2 va = row(2 * t), vb = row(2 * t + 1), vc = row(2 * t + 8), vd = row(2 * t + 9);
+                    four(va.x, vb.x, vc.x, vd.x, acc[0], acc[1]);
+                    four(va.y, vb.y, vc.y, vd.y, acc[2], acc[3]);
+                } else {
+#pragma unroll
+                    for (int sg = 0; sg < D / 128; sg++) {
+                        auto row = [&](uint32_t r2) { return *reinterpret_cast<const uint4*>(v + value_at<D>(r2, sg * 8 + g)); };
+                        const uint4 va = row(2 * t), vb = row(2 * t + 1), vc = row(2 * t + 8), vd = row(2 * t + 9);
+                        four(va.x, vb.x, vc.x, vd.x, acc[sg * 8], acc[sg * 8 + 1]);
+                        four(va.y, vb.y, vc.y, vd.y, acc[sg * 8 + 2], acc[sg * 8 + 3]);
+                        four(va.z, vb.z, vc.z, vd.z, acc[sg * 8 + 4], acc[sg * 8 + 5]);
+                        four(va.w, vb.w, vc.w, vd.w, acc[sg * 8 + 6], acc[sg * 8 + 7]);
+                    }
                 }
             }
         }
-        // The warps meet: statistics, then outputs in units of the values.
+        copy_wait<0>();
+        __syncwarp();  // the ring is free
+        // The warps meet: statistics, then outputs in units of the values, over a warp's own ring.
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (t == 0) s_m[warp * 8 + g] = m, s_l[warp * 8 + g] = l;
         {
-            float* dst = s_acc + warp * 8 * D;
+            float* dst = reinterpret_cast<float*>(ring);
             constexpr int RUN = D == 64 ? 8 : 16;  // dimensions a lane group holds side by side
 #pragma unroll
             for (int i = 0; i < MT; i++) {
@@ -308,62 +433,105 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) paged_attend_kernel
         }
         __syncthreads();
         const bool whole = tile0 == 0 && tile1 == rq.tiles;
-        float* slot = a.partial + (size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * (16 + 8 * D);  // at most one line is begun and not finished, and one finished and not begun
-        auto store = [&](uint32_t row, uint32_t d, float v) {
+        const uint32_t rows = min(8u, rq.n * a.ratio - group * 8);
+        constexpr uint32_t SLOT = 16 + 8 * D;
+        float* slot = a.partial + (size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * SLOT;  // at most one line is begun and not finished, and one finished and not begun
+        auto store = [&](uint32_t row, uint32_t d, float4 v, float sum) {
             const uint32_t i = group * 8 + row, tok = i / a.ratio, head = kvh * a.ratio + i % a.ratio;
-            if (tok >= rq.n) return;
             const unsigned long long p = (unsigned long long)(rq.first + tok) * a.out_stride + (unsigned long long)head * D + d;
-            if (a.out_f16) static_cast<__half*>(a.out)[p] = __float2half_rn(v);
-            else static_cast<float*>(a.out)[p] = v;
+            const float f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+            if (a.out_f16) *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + p) = make_uint2(pack(v.x, v.y), pack(v.z, v.w));
+            else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + p) = v;
         };
-        for (uint32_t e = th; e < 8 * D; e += THREADS) {
+        for (uint32_t e = th * 4; e < rows * D; e += THREADS * 4) {
             const uint32_t row = e / D, d = e % D;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < WARPS; w++) top = fmaxf(top, s_m[w * 8 + row]);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f, v = 0.0f;
+            const float from = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
-                const float f = ex2(s_m[w * 8 + row] - base);
+                const float f = ex2(s_m[w * 8 + row] - from);
+                const float4 x = *reinterpret_cast<const float4*>(raw + S::OFF_RING + w * S::RING + (row * D + d) * 4);
                 sum = fmaf(s_l[w * 8 + row], f, sum);
-                v = fmaf(s_acc[(w * 8 + row) * D + d], f, v);
+                v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
             }
             if (whole) {
-                store(row, d, sum > 0.0f || sum != sum ? v / sum : 0.0f);
+                store(row, d, v, sum);
             } else {
-                slot[16 + e] = v;
+                *reinterpret_cast<float4*>(slot + 16 + e) = v;
                 if (d == 0) slot[row] = top, slot[8 + row] = sum;
             }
         }
         if (!whole) {
-            // Which blocks share this line: block b takes the tiles from floor(total b / blocks) on.
-            const uint32_t b0 = (uint32_t)(((unsigned long long)(line0 + 1) * blocks - 1) / total);
-            const uint32_t b1 = (uint32_t)(((unsigned long long)(line0 + rq.tiles) * blocks - 1) / total);
-            __syncthreads();
-            if (th == 0) {
-                uint32_t* cnt = a.count + b0;  // b0 begins no other line that it leaves unfinished
-                __threadfence();
-                const bool last = atomicAdd(cnt, 1u) == b1 - b0;
-                if (last) *cnt = 0;
-                __threadfence();
-                *s_flag = last;
-            }
-            __syncthreads();
-            if (*s_flag) {
-                for (uint32_t e = th; e < 8 * D; e += THREADS) {
-                    const uint32_t row = e / D, d = e % D;
-                    float top = -INFINITY, sum = 0.0f, v = 0.0f;
-                    for (uint32_t b = b0; b <= b1; b++) {
-                        const float* p = a.partial + (size_t)(2 * b + (b == b0 ? 1 : 0)) * (16 + 8 * D);
-                        const float mb = __ldcg(p + row), now = fmaxf(top, mb), base = now == -INFINITY ? 0.0f : now;
-                        const float f0 = ex2(top - base), f1 = ex2(mb - base);
-                        sum = sum * f0 + __ldcg(p + 8 + row) * f1;
-                        v = v * f0 + __ldcg(p + 16 + e) * f1;
-                        top = now;
-                    }
-                    store(row, d, sum > 0.0f || sum != sum ? v / sum : 0.0f);
+            // Which blocks share this line.
+            const uint32_t b0 = block_of(line0), b1 = block_of(line0 + rq.tiles - 1);
+            auto slot_of = [&](uint32_t b) { return a.partial + (size_t)(2 * b + (b == b0 ? 1 : 0)) * SLOT; };
+            auto arrive = [&](uint32_t* cnt, uint32_t of) {  // whether this block is the last of `of`
+                __syncthreads();
+                if (th == 0) {
+                    uint32_t before_me;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before_me) : "l"(cnt) : "memory");
+                    s_flag = before_me == of - 1;
+                    if (before_me == of - 1) *cnt = 0;
                 }
+                __syncthreads();
+                return s_flag != 0;
+            };
+            // First the set of neighbours this block belongs to, its sum over the first one's own result; then the sets.  With one set that
+            // is all.  A block alone in its set may be the first of another line's set as well, so it takes no counter.
+            const uint32_t count = b1 - b0 + 1;
+            uint32_t first = b0 + (blockIdx.x - b0) / SET * SET, step = 1, of = min(SET, b1 + 1 - first);
+            bool final = count <= SET;
+#pragma unroll 1
+            for (;;) {
+                if (of > 1 && !arrive(final ? a.count + b0 : a.count + 512 + first, of)) break;
+                if (of > 1 || final) {
+#pragma unroll 1
+                    for (uint32_t e = th * 4; e < rows * D; e += THREADS * 4) {
+                        const uint32_t row = e / D, d = e % D;
+                        float top = -INFINITY, sum = 0.0f;
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                        for (uint32_t k = 0; k < of; k += 16) {  // sixteen on their way at a time
+                            float mb[16], lb[16];
+                            float4 x[16];
+#pragma unroll
+                            for (uint32_t u = 0; u < 16; u++) {
+                                mb[u] = -INFINITY, lb[u] = 0.0f, x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (k + u < of) {
+                                    const float* p = slot_of(first + (k + u) * step);
+                                    mb[u] = __ldcg(p + row), lb[u] = __ldcg(p + 8 + row), x[u] = __ldcg(reinterpret_cast<const float4*>(p + 16 + e));
+                                }
+                            }
+                            float now = top;
+#pragma unroll
+                            for (uint32_t u = 0; u < 16; u++) now = fmaxf(now, mb[u]);
+                            const float from = now == -INFINITY ? 0.0f : now, f0 = ex2(top - from);
+                            sum *= f0, v.x *= f0, v.y *= f0, v.z *= f0, v.w *= f0;
+#pragma unroll
+                            for (uint32_t u = 0; u < 16; u++) {
+                                const float f = ex2(mb[u] - from);
+                                sum = fmaf(lb[u], f, sum);
+                                v.x = fmaf(x[u].x, f, v.x), v.y = fmaf(x[u].y, f, v.y), v.z = fmaf(x[u].z, f, v.z), v.w = fmaf(x[u].w, f, v.w);
+                            }
+                            top = now;
+                        }
+                        if (final) {
+                            store(row, d, v, sum);
+                        } else {  // only this thread reads these
+                            *reinterpret_cast<float4*>(slot_of(first) + 16 + e) = v;
+                            if (d == 0) s_wt[0][row] = top, s_wt[1][row] = sum;
+                        }
+                    }
+                }
+                if (final) break;
+                __syncthreads();  // the statistics once every thread has read the old ones
+                if (of > 1 && th < rows) slot_of(first)[th] = s_wt[0][th], slot_of(first)[8 + th] = s_wt[1][th];
+                first = b0, step = SET, of = (count + SET - 1) / SET, final = true;
             }
         }
         __syncthreads();  // the next line writes the queries and the warps' results again
@@ -371,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1) paged_attend_kernel
 }
 
 // Blocks a launch has at most: what is resident at once.
-uint32_t most_blocks(const tb_context* ctx, uint32_t head_dim) { return (uint32_t)ctx->sms * (head_dim <= 128 ? 2 : 1); }
+uint32_t most_blocks(const tb_context* ctx, uint32_t head_dim) { return (uint32_t)ctx->sms * (head_dim == 512 ? Shape<512>::RESIDENT : Shape<64>::RESIDENT); }
 
 int check_attend(const tb_paged_attend* p, const std::string& who, bool few) {
     if (!p) return fail(OUT_OF_RANGE, who + ": null descriptor");
@@ -401,9 +569,9 @@ size_t scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return COUNT_BY
 template <int D>
 cudaError_t run(tb_context* ctx, uint32_t grid, const PagedArgs& a) {
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(paged_attend_kernel<D>, smem_bytes<D>() + (MAX_REQUESTS + 1) * 4, ctx->gpu, done);
+    const cudaError_t e = allow_smem(paged_attend_kernel<D>, Shape<D>::BYTES, ctx->gpu, done);
     if (e != cudaSuccess) return e;
-    return launch_kernel(ctx, paged_attend_kernel<D>, dim3(grid), dim3(THREADS), smem_bytes<D>() + ((size_t)a.requests + 1) * 4, true, a);
+    return launch_kernel(ctx, paged_attend_kernel<D>, dim3(grid), dim3(Shape<D>::THREADS), Shape<D>::BYTES, true, a);
 }
 
 int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
@@ -412,13 +580,13 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
     const uint64_t tiles = ((uint64_t)c.width * c.page + TILE - 1) / TILE;
     if (tiles * c.requests > 0xffffffffull / c.kv_heads / groups) return fail(OUT_OF_RANGE, "tb_attend_paged_q8: more than 2^32 tiles of keys");
     const size_t need = scratch_bytes(ctx, c.head_dim);
-    if (grid > COUNT_BYTES / 4) return fail(UNSUPPORTED, "tb_attend_paged_q8: a GPU of that many multiprocessors");
+    if (grid > COUNT_BYTES / 8) return fail(UNSUPPORTED, "tb_attend_paged_q8: a GPU of that many multiprocessors");
     if (!p.scratch || !aligned(p.scratch, 16) || p.scratch_bytes < need)
         return fail(OUT_OF_RANGE, "tb_attend_paged_q8: needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
     PagedArgs a{};
     a.k = c.k, a.v = c.v, a.ks = c.k_scale, a.vs = c.v_scale, a.table = c.table, a.pages = c.pages, a.shift = log2_of(c.page), a.kv_heads = c.kv_heads;
     a.requests = c.requests, a.width = c.width, a.q = p.q, a.q_stride = p.q_stride, a.q_f16 = p.q_dtype == TB_F16, a.starts = p.starts, a.lengths = p.lengths;
-    a.tokens = p.tokens, a.heads = p.heads, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window > 0x7fffffffu ? 0 : p.window, a.least = 4;
+    a.tokens = p.tokens, a.heads = p.heads, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window > 0x7fffffffu ? 0 : p.window;
     a.scale = p.scale * 1.4426950408889634f, a.out = p.out, a.out_stride = p.out_stride, a.out_f16 = p.out_dtype == TB_F16;
     a.count = static_cast<uint32_t*>(p.scratch);
     a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.scratch) + COUNT_BYTES);
