@@ -486,7 +486,7 @@ typedef struct tb_logits {
     uint32_t rows, vocab;
     uint64_t stride, out_stride;
     const uint32_t* history; /* [rows][history_stride]: the prompt's tokens, then the generated ones */
-    uint32_t history_stride;
+    uint32_t history_stride; /* below 2^20 */
     const uint32_t* prompt;  /* [rows] */
     const uint32_t* total;   /* [rows] */
     const float* repetition; /* [rows] or NULL, as the next two */
@@ -495,7 +495,7 @@ typedef struct tb_logits {
     const uint32_t* bias_token; /* [rows][bias_stride] */
     const float* bias;
     const uint32_t* bias_count; /* [rows] */
-    uint32_t bias_stride;
+    uint32_t bias_stride;       /* at most 1024 */
     const uint32_t* allowed; /* [masks][allowed_stride] words of 32 tokens */
     const uint32_t* mask_of; /* [rows] or NULL */
     uint32_t allowed_stride, masks;

@@ -616,6 +616,46 @@ def test_logits_add_a_tokens_biases_in_the_lists_order(ctx):
             assert bufs[4].download(np.float32, 300)[7] == want
 
 
+def test_logits_of_a_history_picked_against_the_tables(ctx):
+    """Tokens that all fall to one block by its hash, more of them than its table holds: those without room are worked out one by one."""
+    rng = np.random.default_rng(5)
+    vocab, want = 1 << 20, 9000
+    t = np.arange(vocab, dtype=np.uint64)
+    top = ((t * 0x9E3779B1) & 0xFFFFFFFF) >> 16
+    picked = np.concatenate([t[top < 700][:want], t[top < 700][:300]]).astype(np.uint32)  # the smallest hashes: the first block's of up to 93; some twice
+    assert len(picked) == want + 300
+    rng.shuffle(picked)
+    x = rng.standard_normal((1, vocab)).astype(np.float32)
+    bias_token, bias = picked[None, :50].copy(), rng.standard_normal((1, 50)).astype(np.float32)
+    n = len(picked)
+    bufs = [ctx.upload(x), ctx.zeros(4 * vocab), words(ctx, picked), words(ctx, [4000]), words(ctx, [n])] + [ctx.upload(np.array([v], np.float32)) for v in (1.3, 0.2, 0.1)]
+    bufs += [words(ctx, bias_token), ctx.upload(bias), words(ctx, [50])]
+    ctx.logits_adjust(tb.Logits(logits=bufs[0].ptr, out=bufs[1].ptr, dtype=tb.F32, rows=1, vocab=vocab, stride=vocab, out_stride=vocab, history=bufs[2].ptr, history_stride=n,
+                                prompt=bufs[3].ptr, total=bufs[4].ptr, repetition=bufs[5].ptr, frequency=bufs[6].ptr, presence=bufs[7].ptr, bias_token=bufs[8].ptr,
+                                bias=bufs[9].ptr, bias_count=bufs[10].ptr, bias_stride=50))
+    f = lambda v: np.array([v], np.float32)  # noqa: E731
+    y = ref.logits(x, picked[None], [4000], [n], f(1.3), f(0.2), f(0.1), bias_token, bias, [50], None, None)
+    assert np.abs(bufs[1].download(np.float32, vocab)[None] - y).max() <= 64 * 8 * 2.0**-24
+
+
+def test_logits_with_long_histories_and_a_step_before_that_writes_them(ctx):
+    """In place and without a mask only the tokens' kernel runs, right behind a kernel that has written its lists."""
+    rng = np.random.default_rng(6)
+    rows, vocab, n = 3, 5000, 20000
+    h = rng.integers(0, vocab, (rows, n)).astype(np.uint32)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    src, dst = ctx.upload(x), ctx.upload(x)
+    hd, old = words(ctx, h), words(ctx, np.zeros((rows, n)))
+    keep = [words(ctx, [100, 0, n]), words(ctx, [n, n - 7, n]), ctx.upload(np.array([1.1, 1.2, 1.3], np.float32)), ctx.upload(np.array([0.01, 0.02, 0.03], np.float32))]
+    # the lists arrive on the stream right before the call, as uint32 "values" through the stream kernel of an unmasked call
+    ctx.logits_adjust(tb.Logits(logits=hd.ptr, out=old.ptr, dtype=tb.F32, rows=rows, vocab=n, stride=n, out_stride=n))
+    ctx.logits_adjust(tb.Logits(logits=dst.ptr, out=dst.ptr, dtype=tb.F32, rows=rows, vocab=vocab, stride=vocab, out_stride=vocab, history=old.ptr, history_stride=n,
+                                prompt=keep[0].ptr, total=keep[1].ptr, repetition=keep[2].ptr, frequency=keep[3].ptr))
+    y = ref.logits(x, h, [100, 0, n], [n, n - 7, n], np.array([1.1, 1.2, 1.3], np.float32), np.array([0.01, 0.02, 0.03], np.float32), None, None, None, None, None, None)
+    assert np.abs(dst.download(np.float32, x.size).reshape(x.shape) - y).max() <= 64 * 8 * 2.0**-24
+    assert src is not None
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 
 

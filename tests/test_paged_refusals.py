@@ -102,7 +102,7 @@ def test_attention_shapes_without_a_kernel(lib):
 
 @pytest.mark.parametrize("change", [{"logits": None}, {"out": None}, {"dtype": 3}, {"vocab": 0}, {"vocab": 1 << 31}, {"stride": 99}, {"out_stride": 99}, {"total": None},
                                     {"prompt": None}, {"history": None}, {"bias": None}, {"bias_count": None}, {"masks": 0}, {"allowed_stride": 3}, {"logits": AT + 2},
-                                    {"allowed": AT + 2}, {"out_stride": 104}])
+                                    {"allowed": AT + 2}, {"out_stride": 104}, {"bias_stride": 1025}, {"history_stride": 1 << 20}])
 def test_bad_logits(lib, change):
     status, text = call(lib, "tb_logits_adjust", logits(**change))
     assert status == 3 and text.startswith("tb_logits_adjust")
