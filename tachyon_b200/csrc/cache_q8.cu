@@ -7,10 +7,12 @@
 // amax / 127 would round the whole page anew for every new maximum; the price is a step up to twice as wide.  Both quotients are
 // exact, so a code has one right value in any arithmetic.
 //
-// What bounds it: bytes.  A block takes one run (consecutive tokens in consecutive slots of one page) of one head and one of
-// keys and values: a first pass over the rows for the maximum, a second that stores codes, its reads from the L1.  A block looks
-// for the runs that start in its span of tokens; the span grows with the call so that the grid stays near 16 blocks a
-// multiprocessor, a single token a block for a decode step.
+// What bounds it: bytes, and for a call of a few tokens the trips to memory one behind the other (slots, rows and the old scale, codes).
+// A block takes the runs (consecutive tokens in consecutive slots of one page) that start in its span of 8 to 64 tokens, of one head and
+// one of keys and values; it fetches the span's and a page's slots at once and finds the runs in shared memory.  A single run, a
+// prompt's, has the whole block, two have four warps each, up to four have two, and more, a decode step's, a warp each: with a block for
+// every run 1024 single tokens took 57 us instead of 8, with a warp for every run a page of 128 rows would take them one by one.  Rows are
+// fetched for the maximum and, unless the registers hold all of a warp's, once more, from the L1 or L2, for the codes.
 #include "common.cuh"
 #include "paged.h"
 
@@ -18,7 +20,7 @@ namespace tb {
 
 namespace {
 
-constexpr uint32_t WARPS = 4;
+constexpr uint32_t WARPS = 8, MOST_PAGE = 128, LEAST_SPAN = 8, MOST_SPAN = 64;
 
 struct RowsArgs {
     int8_t* codes[2];
@@ -29,35 +31,34 @@ struct RowsArgs {
     uint32_t tokens, kv_heads, shift, slots_end, span, dim;
 };
 
-// Values of a row a lane holds: lane, lane + 32 ... in pieces of four (two for heads of 64).
-template <int D>
+// Values of a row a lane holds: lane, lane + 32 ... in pieces of four (two for heads of 64), as they lie in memory.  ROWS rows at a time:
+// more made no call faster, their code takes longer to arrive than the rows do.
+template <int D, bool F16>
 struct Piece {
-    static constexpr int N = D == 64 ? 2 : 4, TURNS = D == 64 ? 1 : D / 128;
-};
-
-template <int N, bool F16>
-__device__ __forceinline__ void load_piece(const void* base, unsigned long long at, float (&x)[N]) {
-    if constexpr (F16) {
-        const __half* p = static_cast<const __half*>(base) + at;
-        if constexpr (N == 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(p);
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    static constexpr int N = D == 64 ? 2 : 4, TURNS = D == 64 ? 1 : D / 128, WORDS = F16 ? N / 2 : N;
+    static constexpr int ROWS = TURNS * WORDS <= 2 ? 2 : 1;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const void* base, unsigned long long at) {
+        const char* p = static_cast<const char*>(base) + at * (F16 ? 2 : 4);
+        if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (WORDS == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x, w[1] = v.y;
         } else {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(p));
-            x[0] = a.x, x[1] = a.y;
-        }
-    } else {
-        const float* p = static_cast<const float*>(base) + at;
-        if constexpr (N == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-        } else {
-            const float2 a = *reinterpret_cast<const float2*>(p);
-            x[0] = a.x, x[1] = a.y;
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
-}
+    __device__ __forceinline__ float value(int e) const {
+        if constexpr (F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e / 2]));
+            return e & 1 ? f.y : f.x;
+        } else {
+            return __uint_as_float(w[e]);
+        }
+    }
+};
 
 // x * inv (inv a power of two, or 0) to a code: what lies outside (infinities alone do) becomes the nearest end, no number 0.
 __device__ __forceinline__ uint32_t code_of(float x, float inv) {
@@ -66,48 +67,81 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv) {
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(WARPS * 32) cache_append_kernel(const RowsArgs a) {
-    using P = Piece<D>;
+__global__ void __launch_bounds__(WARPS * 32, 4) cache_append_kernel(const RowsArgs a) {
+    using P = Piece<D, F16>;
     __shared__ float top[WARPS];
+    __shared__ uint32_t s_slot[1 + MOST_SPAN + MOST_PAGE];  // of the token before the span, the span's and a page's more
+    __shared__ uint32_t s_start[MOST_SPAN], s_starts;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y, which = blockIdx.z;
     const uint32_t page = 1u << a.shift;
     const void* rows = which ? a.rows[1] : a.rows[0];
+    const uint32_t t_first = blockIdx.x * a.span, t_end = min(t_first + a.span, a.tokens);
     pdl_wait();
-    const uint32_t t_end = min((blockIdx.x + 1) * a.span, a.tokens);
-    for (uint32_t t = blockIdx.x * a.span; t < t_end; t++) {
-        const uint32_t slot = __ldg(a.slots + t);
-        if (slot >= a.slots_end) continue;
-        const uint32_t id = slot >> a.shift, off = slot & (page - 1);
-        if (t > 0 && off > 0 && __ldg(a.slots + t - 1) == slot - 1) continue;  // inside a run that starts before
-        uint32_t m = 1;  // the run's length, at most to the page's end
-        for (bool more = true; more;) {
-            const uint32_t i = m + lane;
-            const bool same = off + i < page && t + i < a.tokens && __ldg(a.slots + t + i) == slot + i;
-            const uint32_t got = __ballot_sync(0xffffffffu, same), len = got == 0xffffffffu ? 32u : (uint32_t)__ffs(~got) - 1;
-            m += len;
-            more = len == 32;
-        }
-        float big = 0.0f;
-        for (uint32_t i = warp; i < m; i += WARPS) {
-            const unsigned long long at = (t + i) * a.token_stride + head * a.head_stride + lane * P::N;
+    for (uint32_t i = threadIdx.x; i < 1 + a.span + page; i += WARPS * 32) {
+        const uint32_t t = t_first + i;  // the token after the one this entry is of
+        s_slot[i] = t > 0 && t - 1 < a.tokens ? __ldg(a.slots + t - 1) : 0xffffffffu;
+    }
+    __syncthreads();
+    if (warp == 0) {  // the runs that start here
+        uint32_t n = 0;
 #pragma unroll
-            for (int k = 0; k < P::TURNS; k++) {
-                float x[P::N];
-                load_piece<P::N, F16>(rows, at + k * 128, x);
-#pragma unroll
-                for (int e = 0; e < P::N; e++) {
-                    const float v = fabsf(x[e]);
-                    if (v <= 3.402823466e38f) big = fmaxf(big, v);  // infinities and NaN do not set the scale
-                }
+        for (uint32_t i0 = 0; i0 < MOST_SPAN; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            bool start = false;
+            if (t_first + i < t_end) {
+                const uint32_t slot = s_slot[1 + i];
+                start = slot < a.slots_end && ((slot & (page - 1)) == 0 || t_first + i == 0 || s_slot[i] != slot - 1);
             }
+            const uint32_t who = __ballot_sync(0xffffffffu, start);
+            if (start) s_start[n + __popc(who & ((1u << lane) - 1))] = i;
+            n += __popc(who);
         }
-        big = warp_max(big);
-        if (lane == 0) top[warp] = big;
-        __syncthreads();
-        big = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        __syncthreads();  // the next run writes `top` again, and nobody may read the old scale after it is replaced
+        if (lane == 0) s_starts = n;
+    }
+    __syncthreads();
+    const uint32_t starts = s_starts;
+    const uint32_t lg = starts <= 1 ? 3 : starts <= 2 ? 2 : starts <= 4 ? 1 : 0, step = 1u << lg;  // warps a run
+    const uint32_t team = warp >> lg, row0 = warp & (step - 1);
+    for (uint32_t run = team; run < starts; run += WARPS >> lg) {
+        const uint32_t* here = s_slot + 1 + s_start[run];
+        const uint32_t t = t_first + s_start[run], slot = here[0], id = slot >> a.shift, off = slot & (page - 1);
         float* sp = (which ? a.scale[1] : a.scale[0]) + (size_t)id * a.kv_heads + head;
         const float was = off > 0 ? *sp : 0.0f;
+        uint32_t m = 0;  // the run's length, at most to the page's end
+        for (uint32_t len = 32; len == 32; m += len) {
+            const bool same = off + m + lane < page && t + m + lane < a.tokens && here[m + lane] == slot + m + lane;
+            const uint32_t got = __ballot_sync(0xffffffffu, same);
+            len = got == 0xffffffffu ? 32u : (uint32_t)__ffs(~got) - 1;
+        }
+        float big = 0.0f;
+        P x[P::ROWS][P::TURNS];
+        const bool held = m <= P::ROWS * step;  // the rows stay in registers
+        auto fetch = [&](uint32_t i) {
+#pragma unroll
+            for (int q = 0; q < P::ROWS; q++)
+#pragma unroll
+                for (int k = 0; k < P::TURNS; k++)
+                    if (i + q * step < m) x[q][k].load(rows, (t + i + q * step) * a.token_stride + head * a.head_stride + lane * P::N + k * 128);
+        };
+#pragma unroll 1
+        for (uint32_t i = row0; i < m; i += P::ROWS * step) {
+            fetch(i);
+#pragma unroll
+            for (int q = 0; q < P::ROWS; q++)
+#pragma unroll
+                for (int k = 0; k < P::TURNS; k++)
+#pragma unroll
+                    for (int e = 0; e < P::N; e++) {
+                        const float v = i + q * step < m ? fabsf(x[q][k].value(e)) : 0.0f;
+                        if (v <= 3.402823466e38f) big = fmaxf(big, v);  // infinities and NaN do not set the scale
+                    }
+        }
+        big = warp_max(big);
+        if (step > 1) {  // a team has one run at most, so `top` is written once
+            if (lane == 0) top[warp] = big;
+            named_bar_sync(1 + team, step * 32);
+            for (uint32_t w = 0; w < step; w++) big = fmaxf(big, top[team * step + w]);
+        }
         // The least power of two with big <= 127 * 2^e, from the bits: big = 2^x * 1.f gives e = x - 6, or x - 5 above 127 / 64.
         float least = 0.0f;
         if (big > 0.0f) {
@@ -121,7 +155,7 @@ __global__ void __launch_bounds__(WARPS * 32) cache_append_kernel(const RowsArgs
         int8_t* codes = (which ? a.codes[1] : a.codes[0]) + ((size_t)id * a.kv_heads + head) * page * D;
         if (off > 0 && s != was) {
             const float ratio = __fmul_rn(was, inv);
-            for (uint32_t i = threadIdx.x; i < off * (D / 4); i += WARPS * 32) {
+            for (uint32_t i = row0 * 32 + lane; i < off * (D / 4); i += step * 32) {
                 uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
                 const uint32_t old = *w;
                 uint32_t now = 0;
@@ -130,22 +164,24 @@ __global__ void __launch_bounds__(WARPS * 32) cache_append_kernel(const RowsArgs
                 *w = now;
             }
         }
-        for (uint32_t i = warp; i < m; i += WARPS) {
-            const unsigned long long at = (t + i) * a.token_stride + head * a.head_stride + lane * P::N;
+#pragma unroll 1
+        for (uint32_t i = row0; i < m; i += P::ROWS * step) {
+            if (!held) fetch(i);
 #pragma unroll
-            for (int k = 0; k < P::TURNS; k++) {
-                float x[P::N];
-                load_piece<P::N, F16>(rows, at + k * 128, x);
-                uint32_t w = 0;
+            for (int q = 0; q < P::ROWS; q++)
 #pragma unroll
-                for (int e = 0; e < P::N; e++) w |= code_of(x[e], inv) << (8 * e);
-                int8_t* dst = codes + (off + i) * D + k * 128 + lane * P::N;
-                if constexpr (P::N == 4) *reinterpret_cast<uint32_t*>(dst) = w;
-                else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
-            }
+                for (int k = 0; k < P::TURNS; k++) {
+                    if (i + q * step >= m) continue;
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int e = 0; e < P::N; e++) w |= code_of(x[q][k].value(e), inv) << (8 * e);
+                    int8_t* dst = codes + (off + i + q * step) * D + k * 128 + lane * P::N;
+                    if constexpr (P::N == 4) *reinterpret_cast<uint32_t*>(dst) = w;
+                    else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
+                }
         }
-        __syncthreads();  // every thread has read the old scale
-        if (threadIdx.x == 0) *sp = s;
+        __syncwarp();  // every lane has read the old scale, and where warps work together, all of them have, before they met
+        if (row0 == 0 && lane == 0) *sp = s;
     }
 }
 
@@ -214,10 +250,9 @@ RowsArgs rows_args(const tb_cache_rows& p) {
 
 int launch_append(tb_context* ctx, const tb_cache_rows& p) {
     RowsArgs a = rows_args(p);
-    const uint64_t blocks = (uint64_t)p.tokens * p.cache.kv_heads * 2, want = (uint64_t)ctx->sms * 16;
-    a.span = (uint32_t)(blocks / want);
-    if (a.span < 1) a.span = 1;
-    if (a.span > p.cache.page) a.span = p.cache.page;
+    const uint64_t each = (uint64_t)p.tokens * p.cache.kv_heads * 2 / ((uint64_t)ctx->sms * 8);  // eight blocks a multiprocessor
+    a.span = LEAST_SPAN;
+    while (a.span < MOST_SPAN && a.span < each) a.span *= 2;
     const dim3 grid((p.tokens + a.span - 1) / a.span, p.cache.kv_heads, 2), block(WARPS * 32);
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());

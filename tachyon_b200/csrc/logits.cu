@@ -230,7 +230,7 @@ int launch_logits(tb_context* ctx, const tb_logits& p) {
     if (!p.bias_token) a.p.bias_stride = 0;
     const uint32_t places = p.vocab + (vec ? 15 / (uint32_t)size : 0);  // in front of a row's first token up to 15 bytes
     // Two blocks a multiprocessor, as far as ranges of 1024 tokens give them; with a long history, which every range walks again, one
-    // (16 rows of 128000 with 32000 tokens: ranges of 4096 22 us, of 8192 19 us).
+    // (16 rows of 128000 with 32000 tokens: ranges of 4096 22 us, of 8192 14.5 us).
     const uint64_t wish = (uint64_t)ctx->sms * (p.history && p.history_stride > 4096 ? 1 : 2);
     while (a.range > LEAST_RANGE && (uint64_t)p.rows * ((places + a.range - 1) / a.range) < wish) a.range /= 2;
     a.ranges = (places + a.range - 1) / a.range;

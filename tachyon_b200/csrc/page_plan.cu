@@ -17,7 +17,7 @@ namespace tb {
 namespace {
 
 constexpr uint32_t THREADS = 512;
-constexpr uint32_t SHARE = 4096;  // tokens a block takes; 8 a thread
+constexpr uint32_t SHARE = 1024;  // tokens a block takes at least; two a thread, each a bisection and two trips to the L2
 constexpr uint32_t ENDS = 0xffffffffu;
 
 struct PlanArgs {
@@ -37,7 +37,7 @@ __device__ __forceinline__ uint32_t owner(const uint32_t* at, uint32_t n, uint32
 }
 
 __global__ void __launch_bounds__(THREADS) page_plan_kernel(const PlanArgs a) {
-    extern __shared__ uint32_t sums[];  // three prefix sums over the requests: new tokens, new pages, pages given back
+    extern __shared__ uint32_t sums[];  // three prefix sums over the requests (new tokens, new pages, pages given back) and their lengths
     __shared__ unsigned long long part[3][THREADS / 32];
     __shared__ uint32_t last;
     const tb_plan& p = a.p;
@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const PlanArgs a) {
     uint32_t* s_tok = sums;
     uint32_t* s_need = sums + n;
     uint32_t* s_back = sums + 2 * n;
+    uint32_t* s_len = sums + 3 * n;
     const unsigned long long most = (unsigned long long)p.width << a.shift;  // positions a request can have
     pdl_wait();
 
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const PlanArgs a) {
         uint32_t t = (uint32_t)before[0], q = (uint32_t)before[1], b = (uint32_t)before[2];
         for (uint32_t r = r0; r < r1; r++) {
             const uint32_t len = __ldcg(p.lengths + r), f = __ldcg(p.fresh + r), add = f == ENDS ? 0 : f, have = (len + p.page - 1) >> a.shift;
-            s_tok[r] = t, s_need[r] = q, s_back[r] = b;
+            s_tok[r] = t, s_need[r] = q, s_back[r] = b, s_len[r] = len;
             if (blockIdx.x == 0) p.starts[r] = t;
             t += add;
             if (f == ENDS) b += have;
@@ -115,13 +116,13 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const PlanArgs a) {
         };
         const uint32_t first = blockIdx.x * THREADS + th, step = gridDim.x * THREADS;
         for (uint32_t t = first; t < tokens; t += step) {
-            const uint32_t r = owner(s_tok, n, t), len = __ldcg(p.lengths + r), pos = len + (t - s_tok[r]), at = pos >> a.shift, have = (len + p.page - 1) >> a.shift;
+            const uint32_t r = owner(s_tok, n, t), len = s_len[r], pos = len + (t - s_tok[r]), at = pos >> a.shift, have = (len + p.page - 1) >> a.shift;
             const uint32_t id = at < have ? __ldcg(p.table + (size_t)r * p.width + at) : page_of(s_need[r] + at - have);
             p.slots[t] = id < p.pages ? (id << a.shift) + (pos & (p.page - 1)) : 0xffffffffu;
             if (p.positions) p.positions[t] = pos;
         }
         for (uint32_t k = first; k < pages; k += step) {
-            const uint32_t r = owner(s_need, n, k), have = (__ldcg(p.lengths + r) + p.page - 1) >> a.shift;
+            const uint32_t r = owner(s_need, n, k), have = (s_len[r] + p.page - 1) >> a.shift;
             p.table[(size_t)r * p.width + have + (k - s_need[r])] = page_of(k);
         }
         for (uint32_t q = count + first; q + pages < top; q += step) p.free_pages[q] = given(q - count);  // given back and not given out
@@ -169,12 +170,12 @@ int launch_plan(tb_context* ctx, const tb_plan& p) {
     static std::atomic<uint64_t> done{0};
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());
-    TB_CUDA(allow_smem(page_plan_kernel, 3 * MAX_REQUESTS * sizeof(uint32_t), ctx->gpu, done));
+    TB_CUDA(allow_smem(page_plan_kernel, 4 * MAX_REQUESTS * sizeof(uint32_t), ctx->gpu, done));
     const PlanArgs a{p, log2_of(p.page)};
     uint32_t grid = (p.max_tokens + SHARE - 1) / SHARE;
     if (grid < 1) grid = 1;
     if (grid > (uint32_t)ctx->sms) grid = (uint32_t)ctx->sms;
-    TB_CUDA(launch_kernel(ctx, page_plan_kernel, dim3(grid), dim3(THREADS), 3 * (size_t)p.requests * sizeof(uint32_t), true, a));
+    TB_CUDA(launch_kernel(ctx, page_plan_kernel, dim3(grid), dim3(THREADS), 4 * (size_t)p.requests * sizeof(uint32_t), true, a));
     return OK;
 }
 
