@@ -31,8 +31,7 @@ inline int check_pages(const tb_pages& c, const std::string& who, bool table) {
     return OK;
 }
 
-// Prefill attention on tcgen05 (paged_prefill.cu) and the shapes it takes; the caller has checked the descriptor.
-bool prefill_paged_supports(const tb_paged_attend& p);
+// Prefill attention on tcgen05 (paged_prefill.cu); the caller has checked the descriptor.
 int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p);
 
 // Makes a context's GPU the current one for a launch and puts the caller's back.

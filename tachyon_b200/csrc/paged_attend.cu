@@ -621,7 +621,6 @@ extern "C" int tb_prefill_paged_q8(tb_context* ctx, const tb_paged_attend* args)
     return entry([&] {
         TB_TRY(check_attend(args, "tb_prefill_paged_q8", false));
         if (!ctx) return fail(OUT_OF_RANGE, "null context");
-        if (args->tokens == 0) return (int)OK;
-        return prefill_paged_supports(*args) ? launch_prefill_paged(ctx, *args) : launch_attend_paged(ctx, *args);
+        return args->tokens == 0 ? (int)OK : launch_prefill_paged(ctx, *args);
     });
 }

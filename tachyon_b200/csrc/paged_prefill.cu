@@ -1,17 +1,17 @@
-// Prefill attention over the paged 8-bit cache on the fifth-generation tensor cores (tb_prefill_paged_q8), heads of 64, 128, 256.
+// Prefill attention over the paged 8-bit cache on the fifth-generation tensor cores (tb_prefill_paged_q8).
 //
 // A block takes 128 query rows of one request and key-value head (row = token * ratio + head) and walks their keys in tiles of KT
 // positions that start at multiples of KT.  Everything the tensor cores read of the queries' side stays in tensor memory: the
 // queries (stored once), the scores S = Q K^T (two buffers), the probabilities (f16, over the scores they came from) and the
 // output, so shared memory only carries keys and values: codes turned to f16 on the way in, a byte read where the f16 cache's
-// kernel reads two.  Eighteen warps:
+// kernel reads two.  Sixteen warps:
 //   warps 0-7    softmax, two threads a query row, half of a tile's keys each: scores out of tensor memory, maximum (the two trade theirs
 //                through shared memory), exponentials, probabilities back into it; the running maximum moves only when a tile passes it by 2^8, and only then the output is rescaled;
-//   warps 8-15   codes to f16: 16 codes a thread and turn, loaded a tile ahead, as 0x6400 | (code + 128) by byte permutes and one packed
+//   warps 8-13   codes to f16: 16 codes a thread and turn, loaded a tile ahead, as 0x6400 | (code + 128) by byte permutes and one packed
 //                fused multiply-add (x * f - 1152 f, exact), stored in the 128-byte swizzle; keys K-major, values as they lie in
 //                the cache, which is the MN-major form of a B operand;
-//   warp 16      one thread issues the products, S of tile i + 1 ahead of P V of tile i;
-//   warp 17      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
+//   warp 14      one thread issues the products, S of tile i + 1 ahead of P V of tile i;
+//   warp 15      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
 // A page's scales are powers of two.  Keys carry theirs relative to the tile's largest, which multiplies the scores; values theirs
 // relative to the largest scale met so far, which multiplies the output at the end (and rescales it when it grows).  Every wait is bounded.
 #include "common.cuh"
@@ -24,27 +24,28 @@ namespace {
 
 using namespace tc;
 
-constexpr int ROWS = 128, SOFT_WARPS = 8, CONVERT_WARPS = 8, GROUP_WARPS = CONVERT_WARPS / 4, MMA_WARP = SOFT_WARPS + CONVERT_WARPS, THREADS = (MMA_WARP + 2) * 32, AHEAD = 8, MOST_PAGES = 8;
+constexpr int ROWS = 128, SOFT_WARPS = 8, CONVERT_WARPS = 6, GROUP_WARPS = 2, GROUPS = CONVERT_WARPS / GROUP_WARPS, MMA_WARP = SOFT_WARPS + CONVERT_WARPS, THREADS = (MMA_WARP + 2) * 32, AHEAD = 8;
 
-template <int D>
+// Heads of D; a block works out VD of the output's dimensions (all of them, but for heads of 512, whose output, queries and scores
+// would take more than the 512 columns: four blocks take 128 each, every one with scores of its own).
+template <int D, int VD>
 struct Shape {
-    static constexpr int KT = D == 256 ? 64 : 128;            // keys a tile
+    static constexpr int KT = D >= 256 ? 64 : 128;            // keys a tile
     static constexpr int KCH = KT * 128;                      // a box of 64 dimensions x KT keys
-    static constexpr int STAGE = D / 64 * KCH;                // a tile's keys (or values)
-    static constexpr int OFF_V = 2 * STAGE, OFF_SUM = 4 * STAGE;
-    static constexpr int COL_O = 0, COL_S = D, COL_Q = D + 2 * KT;  // tensor-memory columns
-    static constexpr uint32_t UNITS = KT * (D / 16) / (GROUP_WARPS * 32);  // sixteen codes each, a thread and tile
+    static constexpr int K_STAGE = D / 64 * KCH, V_STAGE = VD / 64 * KCH;  // a tile's keys and values
+    static constexpr int OFF_V = 2 * K_STAGE, OFF_SUM = OFF_V + 2 * V_STAGE;
+    static constexpr int COL_O = 0, COL_S = VD, COL_Q = VD + 2 * KT;  // tensor-memory columns
     // kind::f16, f32 accumulator, A from tensor memory; N >> 3 at bit 17, M >> 4 at bit 24, bit 16: B is MN-major.
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-    static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+    static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     static_assert(COL_Q + D / 2 <= 512, "tensor memory has 512 columns");
 };
 
-struct Ahead {  // what the last warp finds out about a tile
-    unsigned long long at[MOST_PAGES];   // where the page's first code of the tile lies (page 0 where there is no page: its factors are 0)
-    uint2 kf[MOST_PAGES], vf[MOST_PAGES];  // a page's factor f and -1152 f, two f16 each
-    uint32_t keys[4];                    // bit c: key c of the tile has a page
-    float kref, shrink;                  // multiplies the scores; what the output is multiplied by before this tile
+struct Ahead {  // what the last warp finds out about a tile, for every sixteen of its keys: no page is smaller
+    unsigned long long at[8];  // where their first code lies (in page 0 where there is no page: its factors are 0)
+    uint2 kf[8], vf[8];        // their page's factor f and -1152 f, two f16 each
+    uint32_t keys[4];          // bit c: key c of the tile has a page
+    float kref, shrink;        // multiplies the scores; what the output is multiplied by before this tile
 };
 
 struct Shared {
@@ -72,8 +73,8 @@ struct PrefillArgs {
     int q_f16, out_f16;
 };
 
-// D = A B with A in tensor memory, and the commit of what was issued; the whole warp calls them, the thread with `leader` issues.  Run by
-// one lane under a branch, every product first moves its operands to uniform registers: 75 clocks each instead of the product's own time.
+// D = A B with A in tensor memory, and the commit of what was issued; the whole warp calls them, the thread with `leader` issues.  A
+// product of 128 rows takes 62 clocks with 64 columns, 71 with 128 and 128 with 256.
 __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
@@ -128,6 +129,13 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[64]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Past the L1, which shares its memory with the tiles: with lines kept there a tile of the benchmark's shape took 1.59 us, so 1.39.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // Eight codes as f16 times a factor (f, -1152 f): a 16-byte piece.
 __device__ __forceinline__ uint4 convert8(uint32_t a, uint32_t b, const uint2& factor) {
     const __half2 f = *reinterpret_cast<const __half2*>(&factor.x), off = *reinterpret_cast<const __half2*>(&factor.y);
@@ -142,9 +150,9 @@ __device__ __forceinline__ uint4 convert8(uint32_t a, uint32_t b, const uint2& f
     return out;
 }
 
-template <int D>
+template <int D, int VD>
 __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const PrefillArgs a, uint32_t* status) {
-    using S = Shape<D>;
+    using S = Shape<D, VD>;
     constexpr int KT = S::KT;
     extern __shared__ uint8_t raw_unaligned[];
     uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     if (warp < SOFT_WARPS) {
         // ---- queries, softmax, output: a query row's two threads (warps w and w + 4, tensor-memory lane = row) take half of a tile's
         // keys and half of the dimensions each ---------------------------------------------------------------------------
-        constexpr int HK = KT / 2, HD = D / 2;
+        constexpr int HK = KT / 2, HD = D / 2, HV = VD / 2;  // half of the keys, of the queries' dimensions, of the output's
         const uint32_t quarter = warp & 3, half = warp >> 2, me = 32 * quarter + lane;
         const uint32_t row = row0 + me, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
         const bool valid = tok < n;
@@ -350,9 +358,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                 wait(&sh.pv_done[(i - 1) % AHEAD], ((i - 1) / AHEAD) & 1);  // the output must be at rest
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
+                for (int c = 0; c < HV / 32; c++) {
                     uint32_t o[32];
-                    const uint32_t at = lanes + S::COL_O + half * HD + c * 32;
+                    const uint32_t at = lanes + S::COL_O + half * HV + c * 32;
                     tmem_load(at, o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
@@ -371,11 +379,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         l_run += sh.xch[nt & 1][half ^ 1][me];
         if (ok) {
             const float inv = l_run > 0.0f || l_run != l_run ? sh.vref / l_run : 0.0f;
-            const unsigned long long out_at = (unsigned long long)(first + tok) * a.out_stride + (unsigned long long)head * D + half * HD;
+            const unsigned long long out_at = (unsigned long long)(first + tok) * a.out_stride + (unsigned long long)head * D + blockIdx.y * VD + half * HV;
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; c++) {
+            for (int c = 0; c < HV / 32; c++) {
                 uint32_t o[32];
-                if (nt != 0) tmem_load(lanes + S::COL_O + half * HD + c * 32, o);
+                if (nt != 0) tmem_load(lanes + S::COL_O + half * HV + c * 32, o);
                 if (valid) {
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = nt == 0 || inv == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
@@ -402,46 +410,48 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         }
     } else if (warp < MMA_WARP) {
         // ---- codes to f16 ----------------------------------------------------------------------------------------------
-        // Four groups of two warps: keys of the even tiles, values of the even ones, keys of the odd ones, values of the odd ones.  The fence
-        // in front of the tensor cores waits for a warp's loads in flight as well, so a warp asks for its next tile behind it and the
-        // groups cover each other's trips to the L2.
-        // Unit u of a thread: sixteen codes 64 box + 16 part ... of key key0 + STEP u.  Eight neighbouring lanes take four parts of two
-        // keys, so their 16-byte pieces meet no bank twice.
-        constexpr uint32_t UNITS = S::UNITS, BOXES = D / 64, STEP = GROUP_WARPS * 32 * 16 / D;
-        const uint32_t group = (warp - SOFT_WARPS) / GROUP_WARPS, odd = group >> 1;
-        const bool values = group & 1;
-        const uint32_t me = (th - SOFT_WARPS * 32) % (GROUP_WARPS * 32), part = me & 3, box = (me >> 3) & (BOXES - 1), key0 = (me >> 3) / BOXES * 2 + ((me >> 2) & 1);
-        const int8_t* codes = (values ? a.v : a.k) + box * 64 + part * 16;
-        uint8_t* stage = raw + (values ? S::OFF_V : 0) + odd * S::STAGE + box * S::KCH + key0 * 128;
+        // Three groups of two warps take tasks in turn: task 2 i is tile i's keys, 2 i + 1 its values.  The fence in front of the tensor cores
+        // waits for a warp's loads in flight as well, so a warp asks for its next task behind it and the groups cover each other's trips to
+        // the L2.  (Sixteen warps in all: with more, a thread has 96 registers, and what did not fit cost more than the warps brought.)
+        const uint32_t group = (warp - SOFT_WARPS) / GROUP_WARPS, me = (th - SOFT_WARPS * 32) % (GROUP_WARPS * 32);
+        // A unit of a thread: sixteen codes 64 box + 16 part ... of key key0 + STEP u.  Eight neighbouring lanes take four parts of two keys, so
+        // their 16-byte pieces meet no bank twice.  Keys and values go through the same instructions (heads of 512: keys in four blocks of
+        // columns): with code of their own each the instruction cache, which all the roles share, cost more than the work.
+        constexpr uint32_t BOXES = VD / 64, STEP = GROUP_WARPS * 32 * 16 / VD, UNITS = KT / STEP;
+        static_assert(STEP <= 16, "a unit's keys lie within sixteen");
+        const uint32_t part = me & 3, box = (me >> 3) & (BOXES - 1), key0 = (me >> 3) / BOXES * 2 + ((me >> 2) & 1);
+        const uint32_t from = key0 * D + box * 64 + part * 16, at = box * S::KCH + key0 * 128;
         const uint32_t to0 = ((part * 2) ^ (key0 & 7)) << 4, to1 = ((part * 2 + 1) ^ (key0 & 7)) << 4;
-        uint64_t* full = (values ? sh.v_full : sh.k_full) + odd;
-        const uint32_t mask = min(1u << a.shift, (uint32_t)KT) - 1, shift = min(a.shift, (uint32_t)(KT == 64 ? 6 : 7));  // a page's part of a tile
         uint4 w[UNITS];
-        auto load = [&](uint32_t i) {
-            const Ahead& info = sh.ahead[i % AHEAD];
-            wait(&sh.known[i % AHEAD], (i / AHEAD) & 1);
+        auto load = [&](uint32_t task, uint32_t c) {
+            const Ahead& info = sh.ahead[(task >> 1) % AHEAD];
+            const int8_t* codes = (task & 1 ? a.v + blockIdx.y * VD : a.k + c * VD) + from;
 #pragma unroll
-            for (uint32_t u = 0; u < UNITS; u++) {
-                const uint32_t key = key0 + u * STEP;
-                w[u] = __ldg(reinterpret_cast<const uint4*>(codes + info.at[key >> shift] + (key & mask) * D));
-            }
+            for (uint32_t u = 0; u < UNITS; u++) w[u] = load_once(codes + info.at[u * STEP / 16] + u * STEP % 16 * D);
         };
-        if (odd < nt) load(odd);
-        for (uint32_t i = odd; i < nt; i += 2) {
+        if (group >> 1 < nt) wait(&sh.known[(group >> 1) % AHEAD], 0), load(group, 0);
+        for (uint32_t task = group; task >> 1 < nt; task += GROUPS) {
+            const uint32_t i = task >> 1, values = task & 1, odd = i & 1;
             // S (or P V) of the tile two before has read this buffer.
             if (i >= 2) wait(values ? &sh.pv_done[(i - 2) % AHEAD] : &sh.s_full[odd], values ? ((i - 2) / AHEAD) & 1 : ((i - 2) >> 1) & 1);
             const uint2* factors = values ? sh.ahead[i % AHEAD].vf : sh.ahead[i % AHEAD].kf;
+            uint8_t* stage = raw + (values ? S::OFF_V + odd * S::V_STAGE : odd * S::K_STAGE) + at;
+            for (uint32_t c = 0; c < (D == VD || values ? 1 : D / VD); c++) {
+                if (c != 0) load(task, c);
 #pragma unroll
-            for (uint32_t u = 0; u < UNITS; u++) {
-                const uint2 f = factors[(key0 + u * STEP) >> shift];
-                const uint32_t flip = STEP == 4 && (u & 1) ? 64 : 0;  // four keys on, the swizzle's upper bit turns
-                *reinterpret_cast<uint4*>(stage + (to0 ^ flip) + u * STEP * 128) = convert8(w[u].x, w[u].y, f);
-                *reinterpret_cast<uint4*>(stage + (to1 ^ flip) + u * STEP * 128) = convert8(w[u].z, w[u].w, f);
+                for (uint32_t u = 0; u < UNITS; u++) {
+                    const uint2 f = factors[u * STEP / 16];
+                    const uint32_t flip = (STEP * u & 7) << 4;  // the keys of a thread's units differ in the swizzle's upper bits only
+                    uint8_t* to = stage + c * (BOXES * S::KCH) + u * STEP * 128;
+                    *reinterpret_cast<uint4*>(to + (to0 ^ flip)) = convert8(w[u].x, w[u].y, f);
+                    *reinterpret_cast<uint4*>(to + (to1 ^ flip)) = convert8(w[u].z, w[u].w, f);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(full);
-            if (i + 2 < nt) load(i + 2);
+            if (lane == 0) mbar_arrive((values ? sh.v_full : sh.k_full) + odd);
+            const uint32_t next = task + GROUPS;
+            if (next >> 1 < nt) wait(&sh.known[(next >> 1) % AHEAD], ((next >> 1) / AHEAD) & 1), load(next, 0);
         }
     } else if (warp == MMA_WARP) {
         // ---- products --------------------------------------------------------------------------------------------------
@@ -456,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                 all_wait(&sh.k_full[i & 1], (i >> 1) & 1);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t desc = k_desc + (i & 1) * (S::STAGE >> 4);
+                const uint64_t desc = k_desc + (i & 1) * (S::K_STAGE >> 4);
                 const uint32_t d = tm + S::COL_S + (i & 1) * KT;
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) mma_ts(d, tm + S::COL_Q + k * 8, desc + (((k >> 2) * S::KCH + (k & 3) * 32) >> 4), S::IDESC_S, k > 0 ? 1u : 0u, leader);
@@ -470,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                 all_wait(&sh.v_full[i & 1], (i >> 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t desc = v_desc + (i & 1) * (S::STAGE >> 4);
+                const uint64_t desc = v_desc + (i & 1) * (S::V_STAGE >> 4);
                 const uint32_t p = tm + S::COL_S + (i & 1) * KT;
 #pragma unroll
                 for (int k = 0; k < KT / 16; k++) mma_ts(tm + S::COL_O, p + k * 8, desc + (k * 2048 >> 4), S::IDESC_PV, k > 0 ? 1u : i > 0 ? 1u : 0u, leader);
@@ -484,12 +494,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         __syncwarp();
     } else {
         // ---- the tiles ahead -------------------------------------------------------------------------------------------
-        // A lane a page, as many tiles at once as 32 lanes have pages for; page numbers are asked for two such batches ahead, scales one:
-        // looked up tile by tile, the two trips to the L2 behind one another took longer than everything else about a tile.
-        const uint32_t page = 1u << a.shift, count = page < (uint32_t)KT ? KT / page : 1, tiles = 32 / count;
-        auto page_at = [&](uint32_t b) {  // this lane's page of the batch of tiles that starts with tile b
-            const uint32_t j = tile0 + (b + lane / count) * KT + lane % count * page;
-            const uint32_t id = (j & ~(page - 1)) < end ? __ldg(a.table + (size_t)r * a.width + (j >> a.shift)) : 0xffffffffu;
+        // A lane sixteen keys, as many tiles at once as that makes; page numbers are asked for two such batches ahead, scales one: looked
+        // up tile by tile, the two trips to the L2 behind one another took longer than everything else about a tile.
+        constexpr uint32_t count = KT / 16, tiles = 32 / count;
+        const uint32_t page = 1u << a.shift;
+        auto first_key = [&](uint32_t b) { return tile0 + (b + lane / count) * KT + lane % count * 16; };
+        auto page_at = [&](uint32_t b) {  // the page of this lane's keys in the batch of tiles that starts with tile b
+            const uint32_t j = first_key(b), id = j < end ? __ldg(a.table + (size_t)r * a.width + (j >> a.shift)) : 0xffffffffu;
             return id < a.pages ? id : 0xffffffffu;
         };
         auto scales_at = [&](uint32_t id) {
@@ -512,13 +523,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
             for (uint32_t o = 1; o < count; o <<= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o)), vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
             const uint2 kf = pair(km > 0.0f ? __fdiv_rn(sc.x, km) : 0.0f);
             for (uint32_t t = 0; t < tiles && b + t < nt; t++) {
-                const uint32_t i = b + t, j0 = tile0 + i * KT;
+                const uint32_t i = b + t;
                 const float vnew = fmaxf(vref, __shfl_sync(0xffffffffu, vm, t * count));
                 if (i >= AHEAD) wait(&sh.pv_done[i % AHEAD], (i / AHEAD - 1) & 1);  // nobody reads the entry's old tile any more
                 Ahead& info = sh.ahead[i % AHEAD];
                 if (lane / count == t) {
                     const uint32_t k = lane % count;
-                    info.at[k] = ((((unsigned long long)(id != 0xffffffffu ? id : 0) * a.kv_heads + kvh) << a.shift) + (page > (uint32_t)KT ? j0 & (page - 1) : 0)) * D;
+                    info.at[k] = ((((unsigned long long)(id != 0xffffffffu ? id : 0) * a.kv_heads + kvh) << a.shift) + (first_key(b) & (page - 1))) * D;
                     info.kf[k] = kf, info.vf[k] = pair(vnew > 0.0f ? __fdiv_rn(sc.y, vnew) : 0.0f);
                     if (k == 0) {
                         info.kref = km, info.shrink = vref > 0.0f ? __fdiv_rn(vref, vnew) : 1.0f;
@@ -526,11 +537,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
                     }
                 }
                 if (lane < KT / 32) {
-                    uint32_t keys = 0;
-                    const uint32_t mine = has >> (t * count);
-                    if (page >= (uint32_t)KT) keys = mine & 1u ? 0xffffffffu : 0u;
-                    else if (page >= 32) keys = (mine >> (lane * 32 >> a.shift)) & 1u ? 0xffffffffu : 0u;
-                    else keys = ((mine >> (2 * lane)) & 1u ? 0xffffu : 0u) | ((mine >> (2 * lane + 1)) & 1u ? 0xffff0000u : 0u);  // pages of 16
+                    const uint32_t mine = has >> (t * count + 2 * lane);
+                    const uint32_t keys = (mine & 1u ? 0xffffu : 0u) | (mine & 2u ? 0xffff0000u : 0u);
                     info.keys[lane] = keys;
                 }
                 vref = vnew;
@@ -545,18 +553,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-template <int D>
+template <int D, int VD>
 int run(tb_context* ctx, const PrefillArgs& a, uint32_t grid) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t bytes = 1024 + Shape<D>::OFF_SUM;
-    TB_CUDA(allow_smem(paged_prefill_kernel<D>, bytes + (MAX_REQUESTS + 1) * 4, ctx->gpu, done));
-    TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D>, dim3(grid), dim3(THREADS), bytes + ((size_t)a.requests + 1) * 4, true, a, ctx->status));
+    constexpr size_t bytes = 1024 + Shape<D, VD>::OFF_SUM;
+    static_assert(bytes + (MAX_REQUESTS + 1) * 4 + sizeof(Shared) <= 232448, "over what a block may use");
+    TB_CUDA(allow_smem(paged_prefill_kernel<D, VD>, bytes + (MAX_REQUESTS + 1) * 4, ctx->gpu, done));
+    TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D, VD>, dim3(grid, D / VD), dim3(THREADS), bytes + ((size_t)a.requests + 1) * 4, true, a, ctx->status));
     return OK;
 }
 
 }  // namespace
-
-bool prefill_paged_supports(const tb_paged_attend& p) { return p.cache.head_dim <= 256; }
 
 int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     const tb_pages& c = p.cache;
@@ -572,9 +579,10 @@ int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());
     switch (c.head_dim) {
-        case 64: return run<64>(ctx, a, (uint32_t)grid);
-        case 128: return run<128>(ctx, a, (uint32_t)grid);
-        default: return run<256>(ctx, a, (uint32_t)grid);
+        case 64: return run<64, 64>(ctx, a, (uint32_t)grid);
+        case 128: return run<128, 128>(ctx, a, (uint32_t)grid);
+        case 256: return run<256, 256>(ctx, a, (uint32_t)grid);
+        default: return run<512, 128>(ctx, a, (uint32_t)grid);
     }
 }
 
