@@ -31,8 +31,12 @@ inline int check_pages(const tb_pages& c, const std::string& who, bool table) {
     return OK;
 }
 
-// Prefill attention on tcgen05 (paged_prefill.cu); the caller has checked the descriptor.
+// Attention's scratch begins with the decode kernel's counters, zero between calls; calls of every shape may share it.
+constexpr size_t PAGED_COUNT_BYTES = 4096;
+
+// Prefill attention on tcgen05 (paged_prefill.cu); the caller has checked the descriptor, not the scratch.
 int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p);
+size_t prefill_scratch_bytes(const tb_context* ctx, uint32_t head_dim);
 
 // Makes a context's GPU the current one for a launch and puts the caller's back.
 class DeviceScope {

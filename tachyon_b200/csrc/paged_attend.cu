@@ -18,6 +18,8 @@
 //   O^T = V^T P^T: the scores' accumulator is the B operand's layout as it stands; the weights again go in two f16 parts.  A page's
 //   value scale multiplies the weights, relative to the largest scale met so far, so they stay within f16.
 // Softmax statistics and sums are f32.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -563,8 +565,7 @@ int check_attend(const tb_paged_attend* p, const std::string& who, bool few) {
 }
 
 uint32_t groups_of(uint32_t heads, uint32_t kv_heads, uint32_t most) { return (heads / kv_heads * most + 7) / 8; }
-constexpr size_t COUNT_BYTES = 4096;  // counters first, at one place whatever the shape, so that calls of different shapes may share scratch
-size_t scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return COUNT_BYTES + (size_t)2 * most_blocks(ctx, head_dim) * (16 + 8 * (size_t)head_dim) * 4; }
+size_t scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return PAGED_COUNT_BYTES + (size_t)2 * most_blocks(ctx, head_dim) * (16 + 8 * (size_t)head_dim) * 4; }
 
 template <int D>
 cudaError_t run(tb_context* ctx, uint32_t grid, const PagedArgs& a) {
@@ -580,7 +581,7 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
     const uint64_t tiles = ((uint64_t)c.width * c.page + TILE - 1) / TILE;
     if (tiles * c.requests > 0xffffffffull / c.kv_heads / groups) return fail(OUT_OF_RANGE, "tb_attend_paged_q8: more than 2^32 tiles of keys");
     const size_t need = scratch_bytes(ctx, c.head_dim);
-    if (grid > COUNT_BYTES / 8) return fail(UNSUPPORTED, "tb_attend_paged_q8: a GPU of that many multiprocessors");
+    if (grid > PAGED_COUNT_BYTES / 8) return fail(UNSUPPORTED, "tb_attend_paged_q8: a GPU of that many multiprocessors");
     if (!p.scratch || !aligned(p.scratch, 16) || p.scratch_bytes < need)
         return fail(OUT_OF_RANGE, "tb_attend_paged_q8: needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
     PagedArgs a{};
@@ -589,7 +590,7 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
     a.tokens = p.tokens, a.heads = p.heads, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window > 0x7fffffffu ? 0 : p.window;
     a.scale = p.scale * 1.4426950408889634f, a.out = p.out, a.out_stride = p.out_stride, a.out_f16 = p.out_dtype == TB_F16;
     a.count = static_cast<uint32_t*>(p.scratch);
-    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.scratch) + COUNT_BYTES);
+    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.scratch) + PAGED_COUNT_BYTES);
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());
     switch (c.head_dim) {
@@ -607,7 +608,9 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
 
 using namespace tb;
 
-extern "C" size_t tb_paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return ctx ? scratch_bytes(ctx, head_dim) : 0; }
+extern "C" size_t tb_paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim) {
+    return ctx ? std::max(scratch_bytes(ctx, head_dim), prefill_scratch_bytes(ctx, head_dim)) : 0;
+}
 
 extern "C" int tb_attend_paged_q8(tb_context* ctx, const tb_paged_attend* args) {
     return entry([&] {

@@ -14,6 +14,8 @@
 //   warp 15      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
 // A page's scales are powers of two.  Keys carry theirs relative to the tile's largest, which multiplies the scores; values theirs
 // relative to the largest scale met so far, which multiplies the output at the end (and rescales it when it grows).  Every wait is bounded.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.h"
 #include "tc.cuh"
@@ -25,6 +27,11 @@ namespace {
 using namespace tc;
 
 constexpr int ROWS = 128, SOFT_WARPS = 8, CONVERT_WARPS = 6, GROUP_WARPS = 2, GROUPS = CONVERT_WARPS / GROUP_WARPS, MMA_WARP = SOFT_WARPS + CONVERT_WARPS, THREADS = (MMA_WARP + 2) * 32, AHEAD = 8;
+constexpr uint32_t FEW = 128, LEAST = 6;  // requests among which row tiles are cut; tiles of keys of a piece, at least
+
+// A piece in the scratch: the output [VD / 4][128 rows][4], the rows' maxima, their sums.
+template <int VD>
+constexpr uint32_t PIECE = (VD + 2) * ROWS;
 
 // Heads of D; a block works out VD of the output's dimensions (all of them, but for heads of 512, whose output, queries and scores
 // would take more than the 512 columns: four blocks take 128 each, every one with scores of its own).
@@ -41,6 +48,10 @@ struct Shape {
     static_assert(COL_Q + D / 2 <= 512, "tensor memory has 512 columns");
 };
 
+struct Split {  // what the second kernel reads of a piece: those of a row tile follow one another, the first says how many there are
+    uint32_t parts, row0, kvh, first, n;
+};
+
 struct Ahead {  // what the last warp finds out about a tile, for every sixteen of its keys: no page is smaller
     unsigned long long at[8];  // where their first code lies (in page 0 where there is no page: its factors are 0)
     uint2 kf[8], vf[8];        // their page's factor f and -1152 f, two f16 each
@@ -53,7 +64,8 @@ struct Shared {
     uint32_t tmem;
     float vref;
     Ahead ahead[AHEAD];
-    uint32_t part[THREADS / 32];
+    uint32_t part[THREADS / 32], order[FEW], tiles[FEW];  // the requests by their tiles of keys, most first; those tiles
+    unsigned long long work;
     float xch[2][2][ROWS];  // [tile's parity][half][row]: what a row's two threads trade: each tile their maxima, at the end their sums
 };
 
@@ -71,6 +83,10 @@ struct PrefillArgs {
     uint32_t pages, shift, kv_heads, requests, width, tokens, ratio, most, window;
     float scale;  // softmax scale times log2(e)
     int q_f16, out_f16;
+    uint32_t shares;  // blocks that run at once
+    uint32_t* cut;    // how many pieces there are
+    Split* splits;    // [2 shares]
+    float* partial;   // [2 shares][D / VD] pieces
 };
 
 // D = A B with A in tensor memory, and the commit of what was issued; the whole warp calls them, the thread with `leader` issues.  A
@@ -166,10 +182,52 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         const uint32_t next = a.starts ? __ldg(a.starts + r + 1) : r + 1;
         return next > first && first < a.tokens ? min(min(next - first, a.most), a.tokens - first) : 0u;
     };
-    {  // row tiles before each request
+    // The tiles of keys that a row tile sees: from position `from`, to before position `to`.
+    auto keys = [&](uint32_t row0, uint32_t n, int pos0, uint32_t& from, uint32_t& to) {
+        const int p_first = pos0 + (int)(row0 / a.ratio), p_last = pos0 + (int)min((row0 + ROWS - 1) / a.ratio, n - 1);
+        const int lowest = a.window != 0 && p_first >= (int)a.window ? p_first + 1 - (int)a.window : 0;
+        from = (uint32_t)lowest / KT * KT, to = p_last >= 0 ? (uint32_t)p_last + 1 : 0;
+        return to > from ? (to - from + KT - 1) / KT : 0u;
+    };
+    auto length = [&](uint32_t r) { return min(__ldg(a.lengths + r), a.width << a.shift); };
+    const bool few = a.requests <= FEW;
+    uint32_t most = 0xffffffffu;  // tiles of keys of a piece
+    if (few) {
+        if (th == 0) sh.work = 0;
+        __syncthreads();
+        uint32_t mine = 0;
+        if (th < a.requests) {
+            uint32_t first, from, to;
+            const uint32_t n = new_tokens(th, first), tiles = (n * a.ratio + ROWS - 1) / ROWS;
+            if (tiles != 0) {
+                mine = keys((tiles - 1) * ROWS, n, (int)length(th) - (int)n, from, to);
+                atomicAdd(&sh.work, (unsigned long long)mine * tiles * a.kv_heads);
+            }
+            sh.tiles[th] = mine;
+        }
+        __syncthreads();
+        if (th < a.requests) {
+            uint32_t rank = 0;
+            for (uint32_t o = 0; o < a.requests; o++) {
+                const uint32_t other = sh.tiles[o];
+                rank += other > mine || (other == mine && o < th);
+            }
+            sh.order[rank] = th;
+        }
+        most = (uint32_t)min(max((unsigned long long)LEAST, (sh.work + a.shares - 1) / a.shares), 0xffffffffull);
+        __syncthreads();
+    }
+    auto request = [&](uint32_t i) { return few ? sh.order[i] : i; };
+    auto parts_of = [&](uint32_t r) { return few ? max(1u, (sh.tiles[r] + most - 1) / most) : 1u; };
+    auto pieces = [&](uint32_t i) {
+        uint32_t first;
+        const uint32_t r = request(i);
+        return (new_tokens(r, first) * a.ratio + ROWS - 1) / ROWS * parts_of(r);
+    };
+    {  // pieces before each request
         const uint32_t per = (a.requests + THREADS - 1) / THREADS, r0 = min(th * per, a.requests), r1 = min(r0 + per, a.requests);
-        uint32_t mine = 0, first;
-        for (uint32_t r = r0; r < r1; r++) mine += (new_tokens(r, first) * a.ratio + ROWS - 1) / ROWS;
+        uint32_t mine = 0;
+        for (uint32_t i = r0; i < r1; i++) mine += pieces(i);
         uint32_t x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -180,32 +238,42 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         __syncthreads();
         uint32_t at = x - mine;
         for (uint32_t w = 0; w < warp; w++) at += sh.part[w];
-        for (uint32_t r = r0; r < r1; r++) {
-            s_sum[r] = at;
-            at += (new_tokens(r, first) * a.ratio + ROWS - 1) / ROWS;
-            if (r + 1 == a.requests) s_sum[a.requests] = at;
+        for (uint32_t i = r0; i < r1; i++) {
+            s_sum[i] = at;
+            at += pieces(i);
+            if (i + 1 == a.requests) s_sum[a.requests] = at;
         }
         __syncthreads();
     }
     const uint32_t items = s_sum[a.requests];
+    if (few && blockIdx.x == 0 && blockIdx.y == 0 && th == 0) {
+        uint32_t i = 0;
+        while (i < a.requests && parts_of(request(i)) > 1) i++;
+        *a.cut = min(s_sum[i] * a.kv_heads, gridDim.x);
+    }
     if (blockIdx.x >= items * a.kv_heads) return;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, item = items - 1 - blockIdx.x / a.kv_heads;  // a chunk's last rows, which see most, first
-    uint32_t r = 0;
+    uint32_t i_req = 0;
     {
+        const uint32_t item = blockIdx.x / a.kv_heads;
         uint32_t hi = a.requests;
-        while (hi - r > 1) {
-            const uint32_t mid = (r + hi) >> 1;
-            if (s_sum[mid] <= item) r = mid;
+        while (hi - i_req > 1) {
+            const uint32_t mid = (i_req + hi) >> 1;
+            if (s_sum[mid] <= item) i_req = mid;
             else hi = mid;
         }
     }
-    uint32_t first;
-    const uint32_t n = new_tokens(r, first), len = min(__ldg(a.lengths + r), a.width << a.shift), row0 = (item - s_sum[r]) * ROWS;
-    const int pos0 = (int)len - (int)n;  // the first new token's position; negative when the lengths cannot be
-    const int p_first = pos0 + (int)(row0 / a.ratio), p_last = pos0 + (int)min((row0 + ROWS - 1) / a.ratio, n - 1);
-    const int lowest = a.window != 0 && p_first >= (int)a.window ? p_first + 1 - (int)a.window : 0;
-    const uint32_t tile0 = (uint32_t)lowest / KT * KT, end = p_last >= 0 ? (uint32_t)p_last + 1 : 0;  // keys end before `end`
-    const uint32_t nt = end > tile0 ? (end - tile0 + KT - 1) / KT : 0;
+    // A request's last rows, which see most, first; a row tile's pieces behind one another.
+    const uint32_t r = request(i_req), kvh = blockIdx.x % a.kv_heads, parts = parts_of(r);
+    uint32_t first, tile0, end;
+    const uint32_t n = new_tokens(r, first), place = blockIdx.x / a.kv_heads - s_sum[i_req], part = place % parts;
+    const uint32_t row0 = ((n * a.ratio + ROWS - 1) / ROWS - 1 - place / parts) * ROWS;
+    const int pos0 = (int)length(r) - (int)n;  // the first new token's position; negative when the lengths cannot be
+    uint32_t nt = keys(row0, n, pos0, tile0, end);
+    if (parts > 1) {
+        const uint32_t each = (nt + parts - 1) / parts, t0 = min(part * each, nt);
+        nt = min(each, nt - t0), tile0 += t0 * KT;
+        if (th == 0 && blockIdx.y == 0) a.splits[blockIdx.x] = Split{part == 0 ? parts : 0, row0, kvh, first, n};
+    }
 
     if (th == 0) {
         mbar_init(&sh.q_full, SOFT_WARPS), mbar_init(&sh.drained, 1);
@@ -377,7 +445,23 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
         sh.xch[nt & 1][half][me] = l_run;  // not the slots of the last tile, which the other warp may still read
         meet();
         l_run += sh.xch[nt & 1][half ^ 1][me];
-        if (ok) {
+        if (ok && parts > 1) {  // sums and maximum for the second kernel, the output in columns of four
+            float* dst = a.partial + ((size_t)blockIdx.x * (D / VD) + blockIdx.y) * PIECE<VD>;
+            if (valid && half == 0) dst[VD * ROWS + me] = m_used, dst[(VD + 1) * ROWS + me] = l_run;
+            const float vref = sh.vref;
+#pragma unroll 1
+            for (int c = 0; c < HV / 32 && nt != 0; c++) {
+                uint32_t o[32];
+                tmem_load(lanes + S::COL_O + half * HV + c * 32, o);
+                if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * vref);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(dst)[(half * (HV / 4) + c * 8 + e) * ROWS + me] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+                __syncwarp();
+            }
+        } else if (ok) {
             const float inv = l_run > 0.0f || l_run != l_run ? sh.vref / l_run : 0.0f;
             const unsigned long long out_at = (unsigned long long)(first + tok) * a.out_stride + (unsigned long long)head * D + blockIdx.y * VD + half * HV;
 #pragma unroll 1
@@ -553,6 +637,60 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// Row tiles that were cut: a block adds up the pieces of one of them, always in the order of the keys, a thread a row and sixteen of
+// its columns.
+template <int D, int VD>
+__global__ void __launch_bounds__(ROWS) paged_prefill_join_kernel(const PrefillArgs a) {
+    const uint32_t row = threadIdx.x, col = blockIdx.y * 16;
+    pdl_wait();
+    const uint32_t cut = *a.cut;
+    for (uint32_t b = blockIdx.x; b < cut; b += gridDim.x) {
+        const Split s = a.splits[b];
+        const uint32_t at = s.row0 + row, tok = at / a.ratio, head = s.kvh * a.ratio + at % a.ratio;
+        if (s.parts == 0 || tok >= s.n) continue;
+        float m = -INFINITY, l = 0.0f;
+        float4 o[4] = {};
+#pragma unroll 4
+        for (uint32_t i = 0; i < s.parts; i++) {
+            const float* src = a.partial + ((size_t)(b + i * a.kv_heads) * (D / VD) + blockIdx.z) * PIECE<VD>;
+            const float mi = src[VD * ROWS + row], li = src[(VD + 1) * ROWS + row];
+            float4 x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = reinterpret_cast<const float4*>(src)[(col / 4 + e) * ROWS + row];
+            const float top = fmaxf(m, mi);
+            const bool none = mi == -INFINITY;  // then its output was perhaps not written
+            const float was = top == -INFINITY ? 1.0f : ex2(m - top), is = none ? 0.0f : ex2(mi - top);
+            m = top, l = l * was + li * is;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (none) x[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                o[e].x = o[e].x * was + x[e].x * is, o[e].y = o[e].y * was + x[e].y * is;
+                o[e].z = o[e].z * was + x[e].z * is, o[e].w = o[e].w * was + x[e].w * is;
+            }
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const unsigned long long to = (unsigned long long)(s.first + tok) * a.out_stride + (unsigned long long)head * D + blockIdx.z * VD + col;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (inv == 0.0f) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            o[e].x *= inv, o[e].y *= inv, o[e].z *= inv, o[e].w *= inv;
+        }
+        if (a.out_f16) {
+            __half2 h[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[2 * e] = __floats2half2_rn(o[e].x, o[e].y), h[2 * e + 1] = __floats2half2_rn(o[e].z, o[e].w);
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + to);
+            dst[0] = *reinterpret_cast<uint4*>(h), dst[1] = *reinterpret_cast<uint4*>(h + 4);
+        } else {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + to);
+#pragma unroll
+            for (int e = 0; e < 4; e++) dst[e] = o[e];
+        }
+    }
+}
+
+uint32_t shares_of(const tb_context* ctx, uint32_t head_dim) { return std::max((uint32_t)ctx->sms / (head_dim == 512 ? 4 : 1), 1u); }
+
 template <int D, int VD>
 int run(tb_context* ctx, const PrefillArgs& a, uint32_t grid) {
     static std::atomic<uint64_t> done{0};
@@ -560,10 +698,20 @@ int run(tb_context* ctx, const PrefillArgs& a, uint32_t grid) {
     static_assert(bytes + (MAX_REQUESTS + 1) * 4 + sizeof(Shared) <= 232448, "over what a block may use");
     TB_CUDA(allow_smem(paged_prefill_kernel<D, VD>, bytes + (MAX_REQUESTS + 1) * 4, ctx->gpu, done));
     TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D, VD>, dim3(grid, D / VD), dim3(THREADS), bytes + ((size_t)a.requests + 1) * 4, true, a, ctx->status));
+    if (a.requests <= FEW) TB_CUDA(launch_kernel(ctx, paged_prefill_join_kernel<D, VD>, dim3(a.shares, VD / 16, D / VD), dim3(ROWS), 0, true, a));
     return OK;
 }
 
+// The scratch: the decode kernel's counters, which stay zero; how many pieces; what they are of; the pieces.
+constexpr size_t SPLITS_AT = PAGED_COUNT_BYTES + 16;
+size_t partial_at(uint32_t shares) { return SPLITS_AT + ((size_t)2 * shares * sizeof(Split) + 15) / 16 * 16; }
+
 }  // namespace
+
+size_t prefill_scratch_bytes(const tb_context* ctx, uint32_t head_dim) {
+    const uint32_t shares = shares_of(ctx, head_dim), parts = head_dim == 512 ? 4 : 1;
+    return partial_at(shares) + (size_t)2 * shares * (head_dim + 2 * parts) * ROWS * 4;
+}
 
 int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     const tb_pages& c = p.cache;
@@ -572,10 +720,18 @@ int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     a.requests = c.requests, a.width = c.width, a.q = p.q, a.q_stride = p.q_stride, a.q_f16 = p.q_dtype == TB_F16, a.starts = p.starts, a.lengths = p.lengths;
     a.tokens = p.tokens, a.ratio = p.heads / c.kv_heads, a.most = p.most, a.window = p.window > 0x7fffffffu ? 0 : p.window, a.scale = p.scale * 1.4426950408889634f;
     a.out = p.out, a.out_stride = p.out_stride, a.out_f16 = p.out_dtype == TB_F16;
+    if ((uint64_t)p.tokens * p.heads > 0x7fffffffull) return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: too many rows for one call");
     // Row tiles: at most one a request that is not full, and no request brings more than `most` tokens.
     const uint64_t full = (uint64_t)p.tokens * a.ratio / ROWS + c.requests, each = (((uint64_t)p.most * a.ratio + ROWS - 1) / ROWS) * c.requests;
-    const uint64_t grid = (full < each ? full : each) * c.kv_heads;
+    a.shares = shares_of(ctx, c.head_dim);
+    const uint64_t grid = (full < each ? full : each) * c.kv_heads + (c.requests <= FEW ? a.shares : 0);  // cutting makes at most as many more
     if (grid > 0x7fffffffull) return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: too many rows for one call");
+    const size_t need = prefill_scratch_bytes(ctx, c.head_dim);
+    if (!p.scratch || !aligned(p.scratch, 16) || p.scratch_bytes < need)
+        return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
+    uint8_t* scratch = static_cast<uint8_t*>(p.scratch);
+    a.cut = reinterpret_cast<uint32_t*>(scratch + PAGED_COUNT_BYTES), a.splits = reinterpret_cast<Split*>(scratch + SPLITS_AT);
+    a.partial = reinterpret_cast<float*>(scratch + partial_at(a.shares));
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());
     switch (c.head_dim) {
