@@ -40,7 +40,8 @@ struct Shape {
     static constexpr int KT = D >= 256 ? 64 : 128;            // keys a tile
     static constexpr int KCH = KT * 128;                      // a box of 64 dimensions x KT keys
     static constexpr int K_STAGE = D / 64 * KCH, V_STAGE = VD / 64 * KCH;  // a tile's keys and values
-    static constexpr int OFF_V = 2 * K_STAGE, OFF_SUM = OFF_V + 2 * V_STAGE;
+    static constexpr int QC = D <= 256 ? D : 128, Q_ROW = QC * 2 + 16;  // dimensions of the queries in shared memory at once, on their way to tensor memory
+    static constexpr int OFF_V = 2 * K_STAGE, OFF_Q = OFF_V + 2 * V_STAGE;  // before the roles begin, the prefix sum over the requests lies there
     static constexpr int COL_O = 0, COL_S = VD, COL_Q = VD + 2 * KT;  // tensor-memory columns
     // kind::f16, f32 accumulator, A from tensor memory; N >> 3 at bit 17, M >> 4 at bit 24, bit 16: B is MN-major.
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
@@ -66,6 +67,8 @@ struct Shared {
     Ahead ahead[AHEAD];
     uint32_t part[THREADS / 32], order[FEW], tiles[FEW];  // the requests by their tiles of keys, most first; those tiles
     unsigned long long work;
+    unsigned long long q_at[ROWS];  // where a row's queries lie, all bits set: nowhere
+    float q_inv[ROWS];              // what they are multiplied by
     float xch[2][2][ROWS];  // [tile's parity][half][row]: what a row's two threads trade: each tile their maxima, at the end their sums
 };
 
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     extern __shared__ uint8_t raw_unaligned[];
     uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
     __shared__ Shared sh;
-    uint32_t* s_sum = reinterpret_cast<uint32_t*>(raw + S::OFF_SUM);  // [requests + 1]: row tiles before each request
+    uint32_t* s_sum = reinterpret_cast<uint32_t*>(raw + S::OFF_Q);  // [requests + 1]: row tiles before each request
     const uint32_t th = threadIdx.x, warp = th >> 5, lane = th & 31;
     pdl_wait();
 
@@ -302,62 +305,74 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     if (warp < SOFT_WARPS) {
         // ---- queries, softmax, output: a query row's two threads (warps w and w + 4, tensor-memory lane = row) take half of a tile's
         // keys and half of the dimensions each ---------------------------------------------------------------------------
-        constexpr int HK = KT / 2, HD = D / 2, HV = VD / 2;  // half of the keys, of the queries' dimensions, of the output's
+        constexpr int HK = KT / 2, HV = VD / 2;  // half of the keys, of the output's dimensions
         const uint32_t quarter = warp & 3, half = warp >> 2, me = 32 * quarter + lane;
         const uint32_t row = row0 + me, tok = row / a.ratio, head = kvh * a.ratio + row % a.ratio;
         const bool valid = tok < n;
         const uint32_t lanes = tmem + ((32 * quarter) << 16);
-        const unsigned long long q_at = (unsigned long long)(first + tok) * a.q_stride + (unsigned long long)head * D + half * HD;
+        const unsigned long long q_at = (unsigned long long)(first + tok) * a.q_stride + (unsigned long long)head * D;
         auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (int)quarter) : "memory"); };  // the row's two warps
-        // The row is scaled by a power of two so that its largest lies in [1, 2): f16 then loses 2^-11 of it whatever its size.
-        float factor = 0.0f;
+        // Queries, from the q tensor to tensor memory: a row's two warps fetch their 32 rows, neighbouring lanes neighbouring pieces, and
+        // pass them through shared memory as f16.  (A thread that reads its own row touches a line of its own with every load.)
+        float factor = a.scale;
         if (nt != 0) {
-            auto eight = [&](int d, float (&x)[8]) {
-                if (!valid) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = 0.0f;
-                } else if (a.q_f16) {
-                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + q_at + d));
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ww[e]));
-                        x[2 * e] = f.x, x[2 * e + 1] = f.y;
-                    }
-                } else {
-                    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + q_at + d);
-                    const float4 f = __ldg(p), h = __ldg(p + 1);
-                    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w, x[4] = h.x, x[5] = h.y, x[6] = h.z, x[7] = h.w;
-                }
-            };
-            float big = 0.0f;
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                eight(d, x);
-#pragma unroll
-                for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
-            }
-            sh.xch[1][half][me] = big;
+            constexpr int QC = S::QC, UNITS = QC / 16, PARTS = QC / 8, HQ = QC / 2;
+            const uint32_t me64 = half * 32 + lane;
+            uint8_t* q_rows = raw + S::OFF_Q + 32 * quarter * S::Q_ROW;
+            sh.q_at[me] = valid ? q_at : ~0ull;
             meet();
-            big = fmaxf(big, sh.xch[1][half ^ 1][me]);
-            const uint32_t expo = min(max(__float_as_uint(big) >> 23, 1u), 253u);
-            const float inv = __uint_as_float((254u - expo) << 23);
-            factor = a.scale * __uint_as_float(expo << 23);
+            if (!a.q_f16) {  // rows are scaled by a power of two so that their largest lies in [1, 2): f16 then loses 2^-11 of it whatever its size
+#pragma unroll 2
+                for (uint32_t x = half; x < 32; x += 2) {
+                    const unsigned long long at = sh.q_at[32 * quarter + x];
+                    float big = 0.0f;
+#pragma unroll
+                    for (int d = 0; d < D; d += 64) {
+                        const float2 v = at != ~0ull ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + at + d) + lane) : make_float2(0.0f, 0.0f);
+                        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    }
+#pragma unroll
+                    for (int o = 16; o != 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    const uint32_t expo = min(max(__float_as_uint(big) >> 23, 1u), 253u);
+                    if (lane == 0) sh.q_inv[32 * quarter + x] = __uint_as_float((254u - expo) << 23);
+                }
+                meet();
+                factor *= __uint_as_float((254u << 23) - __float_as_uint(sh.q_inv[me]));
+            }
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; c++) {
-                uint32_t h[16];
+            for (int c = 0; c < D; c += QC) {
+                if (c != 0) meet();
+                if (a.q_f16) {
+                    uint4 w[UNITS];
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    float x[8];
-                    eight(c * 32 + g * 8, x);
+                    for (int u = 0; u < UNITS; u++) {
+                        const unsigned long long at = sh.q_at[32 * quarter + (u * 64 + me64) / PARTS];
+                        w[u] = at != ~0ull ? __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at + c + me64 % PARTS * 8)) : make_uint4(0, 0, 0, 0);
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const __half2 v = __floats2half2_rn(x[2 * e] * inv, x[2 * e + 1] * inv);
-                        h[g * 4 + e] = *reinterpret_cast<const uint32_t*>(&v);
+                    for (int u = 0; u < UNITS; u++) *reinterpret_cast<uint4*>(q_rows + (u * 64 + me64) / PARTS * S::Q_ROW + me64 % PARTS * 16) = w[u];
+                } else {
+#pragma unroll 4
+                    for (int u = 0; u < UNITS; u++) {
+                        const uint32_t x = (u * 64 + me64) / PARTS;
+                        const unsigned long long at = sh.q_at[32 * quarter + x];
+                        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + c + me64 % PARTS * 8);
+                        const float4 v = at != ~0ull ? __ldg(p) : make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = at != ~0ull ? __ldg(p + 1) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        const float inv = sh.q_inv[32 * quarter + x];
+                        const __half2 h[4] = {__floats2half2_rn(v.x * inv, v.y * inv), __floats2half2_rn(v.z * inv, v.w * inv), __floats2half2_rn(y.x * inv, y.y * inv),
+                                              __floats2half2_rn(y.z * inv, y.w * inv)};
+                        *reinterpret_cast<uint4*>(q_rows + x * S::Q_ROW + me64 % PARTS * 16) = *reinterpret_cast<const uint4*>(h);
                     }
                 }
-                tmem_store16(lanes + S::COL_Q + half * (HD / 2) + c * 16, h);
+                meet();
+                const uint8_t* from = raw + S::OFF_Q + me * S::Q_ROW + half * QC;
+#pragma unroll 1
+                for (int e = 0; e < HQ / 8; e += 4) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(h + 4 * k) = *reinterpret_cast<const uint4*>(from + (e + k) * 16);
+                    tmem_store16(lanes + S::COL_Q + c / 2 + half * (HQ / 2) + e * 4, h);
+                }
             }
             tmem_wait_st();
         }
@@ -694,10 +709,11 @@ uint32_t shares_of(const tb_context* ctx, uint32_t head_dim) { return std::max((
 template <int D, int VD>
 int run(tb_context* ctx, const PrefillArgs& a, uint32_t grid) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t bytes = 1024 + Shape<D, VD>::OFF_SUM;
-    static_assert(bytes + (MAX_REQUESTS + 1) * 4 + sizeof(Shared) <= 232448, "over what a block may use");
-    TB_CUDA(allow_smem(paged_prefill_kernel<D, VD>, bytes + (MAX_REQUESTS + 1) * 4, ctx->gpu, done));
-    TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D, VD>, dim3(grid, D / VD), dim3(THREADS), bytes + ((size_t)a.requests + 1) * 4, true, a, ctx->status));
+    using S = Shape<D, VD>;
+    constexpr size_t bytes = 1024 + S::OFF_Q + std::max<size_t>(ROWS * S::Q_ROW, (MAX_REQUESTS + 1) * 4);
+    static_assert(bytes + sizeof(Shared) <= 232448, "over what a block may use");
+    TB_CUDA(allow_smem(paged_prefill_kernel<D, VD>, bytes, ctx->gpu, done));
+    TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D, VD>, dim3(grid, D / VD), dim3(THREADS), bytes, true, a, ctx->status));
     if (a.requests <= FEW) TB_CUDA(launch_kernel(ctx, paged_prefill_join_kernel<D, VD>, dim3(a.shares, VD / 16, D / VD), dim3(ROWS), 0, true, a));
     return OK;
 }
