@@ -447,8 +447,8 @@ TB_API int tb_cache_read_q8(tb_context* ctx, const tb_cache_rows* args);
  * tb_attend_paged_q8: for few rows, most * heads / kv_heads <= 64: a decode step.  f32 accuracy (queries and probabilities are
  * multiplied in two f16 parts).
  * tb_prefill_paged_q8: for chunks of a prompt.  Queries and probabilities are rounded to f16 as in tb_prefill_attend.
- * scratch: tb_paged_scratch_bytes bytes, zero before the first launch; calls may share it as long as they do not overlap
- * (whatever their shapes).
+ * scratch: tb_paged_scratch_bytes bytes for the head size, zero before the first launch; calls of both kinds and of any shape may
+ * share it as long as they do not overlap.
  */
 typedef struct tb_paged_attend {
     tb_pages cache;
@@ -483,7 +483,7 @@ typedef struct tb_logits {
     const void* logits;    /* [rows][vocab], stride values from row to row */
     void* out;
     int dtype;             /* TB_F32 or TB_F16, of both */
-    uint32_t rows, vocab;
+    uint32_t rows, vocab;    /* vocab at most 2^30 */
     uint64_t stride, out_stride;
     const uint32_t* history; /* [rows][history_stride]: the prompt's tokens, then the generated ones */
     uint32_t history_stride; /* below 2^20 */

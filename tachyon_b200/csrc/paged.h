@@ -38,6 +38,10 @@ constexpr size_t PAGED_COUNT_BYTES = 4096;
 int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p);
 size_t prefill_scratch_bytes(const tb_context* ctx, uint32_t head_dim);
 
+// What both take of it (paged_attend.cu), and the check that a call brings it.
+size_t paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim);
+int check_scratch(const tb_context* ctx, const tb_paged_attend& p, const std::string& who);
+
 // Makes a context's GPU the current one for a launch and puts the caller's back.
 class DeviceScope {
   public:

@@ -580,10 +580,8 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
     const uint32_t groups = groups_of(p.heads, c.kv_heads, p.most), grid = most_blocks(ctx, c.head_dim);
     const uint64_t tiles = ((uint64_t)c.width * c.page + TILE - 1) / TILE;
     if (tiles * c.requests > 0xffffffffull / c.kv_heads / groups) return fail(OUT_OF_RANGE, "tb_attend_paged_q8: more than 2^32 tiles of keys");
-    const size_t need = scratch_bytes(ctx, c.head_dim);
     if (grid > PAGED_COUNT_BYTES / 8) return fail(UNSUPPORTED, "tb_attend_paged_q8: a GPU of that many multiprocessors");
-    if (!p.scratch || !aligned(p.scratch, 16) || p.scratch_bytes < need)
-        return fail(OUT_OF_RANGE, "tb_attend_paged_q8: needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
+    TB_TRY(check_scratch(ctx, p, "tb_attend_paged_q8"));
     PagedArgs a{};
     a.k = c.k, a.v = c.v, a.ks = c.k_scale, a.vs = c.v_scale, a.table = c.table, a.pages = c.pages, a.shift = log2_of(c.page), a.kv_heads = c.kv_heads;
     a.requests = c.requests, a.width = c.width, a.q = p.q, a.q_stride = p.q_stride, a.q_f16 = p.q_dtype == TB_F16, a.starts = p.starts, a.lengths = p.lengths;
@@ -604,13 +602,19 @@ int launch_attend_paged(tb_context* ctx, const tb_paged_attend& p) {
 
 }  // namespace
 
+size_t paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return std::max(scratch_bytes(ctx, head_dim), prefill_scratch_bytes(ctx, head_dim)); }
+
+int check_scratch(const tb_context* ctx, const tb_paged_attend& p, const std::string& who) {
+    const size_t need = paged_scratch_bytes(ctx, p.cache.head_dim);
+    if (p.scratch && aligned(p.scratch, 16) && p.scratch_bytes >= need) return OK;
+    return fail(OUT_OF_RANGE, who + ": needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
+}
+
 }  // namespace tb
 
 using namespace tb;
 
-extern "C" size_t tb_paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim) {
-    return ctx ? std::max(scratch_bytes(ctx, head_dim), prefill_scratch_bytes(ctx, head_dim)) : 0;
-}
+extern "C" size_t tb_paged_scratch_bytes(const tb_context* ctx, uint32_t head_dim) { return ctx ? paged_scratch_bytes(ctx, head_dim) : 0; }
 
 extern "C" int tb_attend_paged_q8(tb_context* ctx, const tb_paged_attend* args) {
     return entry([&] {

@@ -742,9 +742,7 @@ int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     a.shares = shares_of(ctx, c.head_dim);
     const uint64_t grid = (full < each ? full : each) * c.kv_heads + (c.requests <= FEW ? a.shares : 0);  // cutting makes at most as many more
     if (grid > 0x7fffffffull) return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: too many rows for one call");
-    const size_t need = prefill_scratch_bytes(ctx, c.head_dim);
-    if (!p.scratch || !aligned(p.scratch, 16) || p.scratch_bytes < need)
-        return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: needs " + std::to_string(need) + " bytes of 16-byte aligned scratch (tb_paged_scratch_bytes)");
+    TB_TRY(check_scratch(ctx, p, "tb_prefill_paged_q8"));
     uint8_t* scratch = static_cast<uint8_t*>(p.scratch);
     a.cut = reinterpret_cast<uint32_t*>(scratch + PAGED_COUNT_BYTES), a.splits = reinterpret_cast<Split*>(scratch + SPLITS_AT);
     a.partial = reinterpret_cast<float*>(scratch + partial_at(a.shares));

@@ -528,6 +528,79 @@ def test_prefill_longer(ctx, D, ratio, spread):
     attend_case(ctx, D, 64, 1, ratio, [1500, 260], [200, 257], 0, np.float16, np.float32, prefill=True, spread=spread)
 
 
+@pytest.mark.parametrize("D,page,kvh,ratio", [(64, 16, 2, 4), (128, 64, 1, 7), (256, 32, 2, 4), (512, 128, 1, 4)])
+@pytest.mark.parametrize("window", [0, 1333])
+@pytest.mark.parametrize("q_kind,out_kind", [(np.float16, np.float16), (np.float32, np.float32)])
+def test_prefill_of_few_rows_behind_many_keys(ctx, D, page, kvh, ratio, window, q_kind, out_kind):
+    """Row tiles whose keys are cut into pieces; some see less than there are pieces."""
+    attend_case(ctx, D, page, kvh, ratio, [6001, 2111, 40, 5], [60, 7, 33, 5], window, q_kind, out_kind, prefill=True)
+
+
+def test_prefill_over_pieces_without_pages(ctx):
+    """Pieces none of whose keys has a page, in front, in the middle and everywhere; lengths below the number of new tokens."""
+    rng = np.random.default_rng(13)
+    D, page, kvh, ratio, pages = 128, 64, 1, 4, 70
+    cache = Cache(ctx, pages, kvh, page, D, 3)
+    lengths, new = [4000, 4000, 4000, 3], [40, 40, 40, 9]
+    table = rng.integers(0, pages, (4, 63)).astype(np.uint32)
+    table[0, :30] = 0xFFFFFFFF
+    table[1, 20:50] = pages
+    table[2, :] = 0xFFFFFFFF
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((int(starts[-1]), kvh * ratio, D)).astype(np.float16)
+    got = run_attend(ctx, cache, q, np.float16, table, starts, lengths, 0, 0.1, np.float32, 40, True)
+    want, size, vmax = ref.attend(q.astype(np.float64), cache.k, cache.ks, cache.v, cache.vs, table, starts, lengths, 0, 0.1, page)
+    assert np.all(np.abs(got - want) <= attention_bound(want, size, vmax, D, 4000, False, True))
+    assert np.all(got[80:120] == 0) and np.all(got[120:126] == 0)
+
+
+@pytest.mark.parametrize("requests", [128, 129])
+def test_prefill_of_many_requests(ctx, requests):
+    """Up to 128 requests are ordered by their lengths; idle ones among them."""
+    rng = np.random.default_rng(requests)
+    lengths, new = rng.integers(20, 700, requests), rng.integers(0, 20, requests)
+    attend_case(ctx, 64, 16, 1, 4, lengths.tolist(), new.tolist(), 0, np.float16, np.float32, prefill=True)
+
+
+@pytest.mark.parametrize("kind,sizes", [(np.float16, (2.0**-20, 2.0**-10, 2.0**10)), (np.float32, (1e-30, 1e-8, 1e8, 1e30))])
+def test_prefill_queries_of_any_size(ctx, kind, sizes):
+    """f32 queries are scaled before they are rounded, f16 ones are taken as they are, those below the normal range among them."""
+    D, page = 64, 16
+    cache = Cache(ctx, 4, 1, page, D, 3)
+    rng = np.random.default_rng(1)
+    table = np.arange(4, dtype=np.uint32)[None]
+    base = rng.standard_normal((3, 2, D)).astype(kind)
+    for f in sizes:
+        q = base * kind(f)
+        scale = np.float32(1 / f)
+        got = run_attend(ctx, cache, q, kind, table, [0, 3], [50], 0, scale, np.float32, 3, True)
+        want, size, vmax = ref.attend(q.astype(np.float64), cache.k, cache.ks, cache.v, cache.vs, table, [0, 3], [50], 0, float(scale), page)
+        bound = attention_bound(want, size, vmax, D, 50, False, True) + (2 * vmax * size * 2.0**-11 if kind == np.float32 else 0)
+        assert np.all(np.abs(got - want) <= bound)
+
+
+def test_prefill_gives_the_same_bits_and_shares_scratch(ctx):
+    """Twice the same calls through one scratch, a decode step's between them."""
+    scratch = ctx.zeros(max(ctx.paged_scratch_bytes(D) for D in (64, 128, 256, 512)))
+    outs = []
+    for _ in range(2):
+        for D, kvh, lengths, new, prefill in ((128, 2, [5000, 300], [50, 200], True), (256, 1, [9000], [1], False), (512, 1, [3000], [9], True), (64, 2, [700] * 9, [70] * 9, True)):
+            cache = Cache(ctx, 150, kvh, 64, D, 1)
+            table = tables(np.random.default_rng(3), lengths, 64, 150, 150)
+            q = np.random.default_rng(4).standard_normal((sum(new), kvh * 4, D)).astype(np.float32)
+            outs.append(run_attend(ctx, cache, q, np.float32, table, np.concatenate([[0], np.cumsum(new)]), lengths, 0, 0.1, np.float32, max(new), prefill, scratch=scratch))
+    for a, b in zip(outs[:4], outs[4:]):
+        assert np.array_equal(a, b)
+
+
+def test_prefill_needs_its_scratch(ctx):
+    cache = Cache(ctx, 2, 1, 16, 64, 1)
+    small = ctx.zeros(ctx.paged_scratch_bytes(64) - 16)
+    with pytest.raises(tb.Error, match="tb_paged_scratch_bytes") as e:
+        run_attend(ctx, cache, np.zeros((1, 1, 64), np.float32), np.float32, np.zeros((1, 1), np.uint32), [0, 1], [3], 0, 1.0, np.float32, 1, True, scratch=small)
+    assert e.value.status == 3
+
+
 # ---- logits ----------------------------------------------------------------------------------------------------------
 
 
