@@ -1,12 +1,15 @@
 // Prefill attention over the paged 8-bit cache on the fifth-generation tensor cores (tb_prefill_paged_q8).
 //
-// A block takes 128 query rows of one request and key-value head (row = token * ratio + head) and walks their keys in tiles of KT
-// positions that start at multiples of KT.  Everything the tensor cores read of the queries' side stays in tensor memory: the
-// queries (stored once), the scores S = Q K^T (two buffers), the probabilities (f16, over the scores they came from) and the
-// output, so shared memory only carries keys and values: codes turned to f16 on the way in, a byte read where the f16 cache's
-// kernel reads two.  Sixteen warps:
+// out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) q.k_j - m): 4 D operations a query row and key.  A row tile is 128 query rows
+// of one request and key-value head (row = token * ratio + head); a block walks its keys in tiles of KT positions that start at
+// multiples of KT.  Where there are fewer row tiles than multiprocessors the keys are cut into pieces, one a block; a first kernel of
+// one block says who does what, a last one adds the pieces up.  Everything the tensor cores read of the queries' side stays in tensor
+// memory: the queries (stored once), the scores S = Q K^T (two buffers), the probabilities (f16, over the scores they came from) and
+// the output, so shared memory only carries keys and values: codes turned to f16 on the way in, a byte read where an f16 cache takes
+// two.  Sixteen warps:
 //   warps 0-7    softmax, two threads a query row, half of a tile's keys each: scores out of tensor memory, maximum (the two trade theirs
-//                through shared memory), exponentials, probabilities back into it; the running maximum moves only when a tile passes it by 2^8, and only then the output is rescaled;
+//                through shared memory), exponentials, probabilities back into it; the running maximum moves only when a tile passes it
+//                by 2^8, and only then the output is rescaled;
 //   warps 8-13   codes to f16: 16 codes a thread and turn, loaded a tile ahead, as 0x6400 | (code + 128) by byte permutes and one packed
 //                fused multiply-add (x * f - 1152 f, exact), stored in the 128-byte swizzle; keys K-major, values as they lie in
 //                the cache, which is the MN-major form of a B operand;
@@ -14,6 +17,14 @@
 //   warp 15      looks up the pages of the tiles ahead: page numbers, the pages' factors, which keys have a page at all.
 // A page's scales are powers of two.  Keys carry theirs relative to the tile's largest, which multiplies the scores; values theirs
 // relative to the largest scale met so far, which multiplies the output at the end (and rescales it when it grows).  Every wait is bounded.
+//
+// Measured, 148 row tiles over 7.6 to 10 thousand keys: heads of 256 216 us (793 TFLOP/s, 48 % of the tensor cores' measured 1654), of
+// 128 120 us (714), of 64 111 us (387).  What bounds it: with heads of 256 the products' own issue, 2400 clocks a tile of 64 keys of
+// which S takes 1000 (a product of 64 columns takes no less than half of one of 256) and P V 520, and the waits between them; with heads
+// of 128 and 64 the softmax, 2600 clocks a tile of 128 keys, 1400 of them exponentials and their conversion.  Heads of 512 work S out four
+// times, once for each 128 dimensions of the output: 1412 us.  Tried without gain: a third of the exponentials by a polynomial, packed
+// multiply-adds, registers moved between the roles, 20 warps (what did not fit the registers cost more), P V ahead of the next S, a
+// block that goes on to its next piece (the same work with the loop's registers on top: 5 to 20 % slower).
 #include <algorithm>
 
 #include "common.cuh"
@@ -27,7 +38,8 @@ namespace {
 using namespace tc;
 
 constexpr int ROWS = 128, SOFT_WARPS = 8, CONVERT_WARPS = 6, GROUP_WARPS = 2, GROUPS = CONVERT_WARPS / GROUP_WARPS, MMA_WARP = SOFT_WARPS + CONVERT_WARPS, THREADS = (MMA_WARP + 2) * 32, AHEAD = 8;
-constexpr uint32_t FEW = 128, LEAST = 6;  // requests among which row tiles are cut; tiles of keys of a piece, at least
+constexpr uint32_t FEW = 128;    // requests up to which they are ordered and their row tiles cut: more have row tiles enough
+constexpr uint32_t LEAST = 384;  // keys of a piece, at least: with twice as many 100 tokens behind 8092 (heads of 128) took 39 us instead of 30, with half as many 60 behind 8132 (256) 35 instead of 32
 
 // A piece in the scratch: the output [VD / 4][128 rows][4], the rows' maxima, their sums.
 template <int VD>
@@ -41,12 +53,17 @@ struct Shape {
     static constexpr int KCH = KT * 128;                      // a box of 64 dimensions x KT keys
     static constexpr int K_STAGE = D / 64 * KCH, V_STAGE = VD / 64 * KCH;  // a tile's keys and values
     static constexpr int QC = D <= 256 ? D : 128, Q_ROW = QC * 2 + 16;  // dimensions of the queries in shared memory at once, on their way to tensor memory
-    static constexpr int OFF_V = 2 * K_STAGE, OFF_Q = OFF_V + 2 * V_STAGE;  // before the roles begin, the prefix sum over the requests lies there
+    static constexpr int OFF_V = 2 * K_STAGE, OFF_Q = OFF_V + 2 * V_STAGE, BYTES = 1024 + OFF_Q + ROWS * Q_ROW;
     static constexpr int COL_O = 0, COL_S = VD, COL_Q = VD + 2 * KT;  // tensor-memory columns
     // kind::f16, f32 accumulator, A from tensor memory; N >> 3 at bit 17, M >> 4 at bit 24, bit 16: B is MN-major.
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     static_assert(COL_Q + D / 2 <= 512, "tensor memory has 512 columns");
+};
+
+struct Row {  // a request, in the order the blocks take them
+    uint32_t r, first, n, len, parts;  // its first row of q, its new tokens, its length, the pieces its row tiles are cut into
+    uint32_t unused[3];
 };
 
 struct Split {  // what the second kernel reads of a piece: those of a row tile follow one another, the first says how many there are
@@ -65,8 +82,8 @@ struct Shared {
     uint32_t tmem;
     float vref;
     Ahead ahead[AHEAD];
-    uint32_t part[THREADS / 32], order[FEW], tiles[FEW];  // the requests by their tiles of keys, most first; those tiles
-    unsigned long long work;
+    Row row;           // the block's request
+    uint32_t place;    // which of its pieces
     unsigned long long q_at[ROWS];  // where a row's queries lie, all bits set: nowhere
     float q_inv[ROWS];              // what they are multiplied by
     float xch[2][2][ROWS];  // [tile's parity][half][row]: what a row's two threads trade: each tile their maxima, at the end their sums
@@ -86,8 +103,10 @@ struct PrefillArgs {
     uint32_t pages, shift, kv_heads, requests, width, tokens, ratio, most, window;
     float scale;  // softmax scale times log2(e)
     int q_f16, out_f16;
-    uint32_t shares;  // blocks that run at once
-    uint32_t* cut;    // how many pieces there are
+    uint32_t shares, blocks;  // blocks that run at once; that are launched
+    uint32_t* head;   // how many blocks have a piece of a row tile that was cut, how many have one at all
+    uint32_t* before; // [requests]: pieces of a key-value head before each request, in the order of `rows`
+    Row* rows;        // [requests]
     Split* splits;    // [2 shares]
     float* partial;   // [2 shares][D / VD] pieces
 };
@@ -169,6 +188,108 @@ __device__ __forceinline__ uint4 convert8(uint32_t a, uint32_t b, const uint2& f
     return out;
 }
 
+// The tiles of keys that a row tile sees: from position `from`, to before position `to`.
+template <int KT>
+__device__ __forceinline__ uint32_t keys_of(const PrefillArgs& a, uint32_t row0, uint32_t n, int pos0, uint32_t& from, uint32_t& to) {
+    const int p_first = pos0 + (int)(row0 / a.ratio), p_last = pos0 + (int)min((row0 + ROWS - 1) / a.ratio, n - 1);
+    const int lowest = a.window != 0 && p_first >= (int)a.window ? p_first + 1 - (int)a.window : 0;
+    from = (uint32_t)lowest / KT * KT, to = p_last >= 0 ? (uint32_t)p_last + 1 : 0;
+    return to > from ? (to - from + KT - 1) / KT : 0u;
+}
+
+// What each block will do.  Up to FEW requests are taken longest first, so that the last blocks to start are short ones, and their row
+// tiles are cut along the keys: into pieces of an even share of all the work, and where that leaves more pieces than run at once although
+// there are fewer row tiles, into the longest pieces that do not.  (By every block for itself this took 7 us a block.)
+template <int KT>
+__global__ void __launch_bounds__(THREADS) paged_prefill_plan_kernel(const PrefillArgs a) {
+    __shared__ uint32_t part[THREADS / 32], order[FEW], seen[FEW], sum;
+    __shared__ unsigned long long work;
+    const uint32_t th = threadIdx.x, lane = th & 31;
+    pdl_wait();
+    auto row_of = [&](uint32_t r) {
+        Row x{r, a.starts ? __ldg(a.starts + r) : r, 0, min(__ldg(a.lengths + r), a.width << a.shift), 1, {0, 0, 0}};
+        const uint32_t next = a.starts ? __ldg(a.starts + r + 1) : r + 1;
+        if (next > x.first && x.first < a.tokens) x.n = min(min(next - x.first, a.most), a.tokens - x.first);
+        return x;
+    };
+    auto tiles_of = [&](const Row& x) { return (x.n * a.ratio + ROWS - 1) / ROWS; };
+    auto total = [&](uint32_t x) {  // over the block
+        for (int o = 16; o != 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (th == 0) sum = 0;
+        __syncthreads();
+        if (lane == 0 && x != 0) atomicAdd(&sum, x);
+        __syncthreads();
+        x = sum;
+        __syncthreads();
+        return x;
+    };
+    const bool few = a.requests <= FEW;
+    uint32_t most = 0xffffffffu;  // tiles of keys of a piece
+    if (few) {
+        if (th == 0) work = 0;
+        __syncthreads();
+        uint32_t mine = 0, tiles = 0;  // tiles of keys of a request's last row tile, which sees most; its row tiles
+        if (th < a.requests) {
+            uint32_t from, to;
+            const Row x = row_of(th);
+            tiles = tiles_of(x);
+            if (tiles != 0) {
+                mine = keys_of<KT>(a, (tiles - 1) * ROWS, x.n, (int)x.len - (int)x.n, from, to);
+                atomicAdd(&work, (unsigned long long)mine * tiles * a.kv_heads);
+            }
+            seen[th] = mine;
+        }
+        __syncthreads();
+        if (th < a.requests) {
+            uint32_t rank = 0;
+#pragma unroll 8
+            for (uint32_t o = 0; o < a.requests; o++) {
+                const uint32_t other = seen[o];
+                rank += other > mine || (other == mine && o < th);
+            }
+            order[rank] = th;
+        }
+        most = (uint32_t)min(max((unsigned long long)(LEAST / KT), (work + a.shares - 1) / a.shares), 0x7fffffffull);
+        if (total(tiles) * (unsigned long long)a.kv_heads <= a.shares)
+            while (total(tiles * max(1u, (mine + most - 1) / most)) * (unsigned long long)a.kv_heads > a.shares) most += (most + 15) / 16;
+    }
+    auto row_at = [&](uint32_t i) {
+        Row x = row_of(few ? order[i] : i);
+        if (few) x.parts = max(1u, (seen[x.r] + most - 1) / most);
+        return x;
+    };
+    const uint32_t per = (a.requests + THREADS - 1) / THREADS, r0 = min(th * per, a.requests), r1 = min(r0 + per, a.requests);
+    uint32_t mine = 0;
+    for (uint32_t i = r0; i < r1; i++) {
+        const Row x = row_at(i);
+        mine += tiles_of(x) * x.parts;
+    }
+    uint32_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+    }
+    if (lane == 31) part[th >> 5] = x;
+    __syncthreads();
+    uint32_t at = x - mine, cut = 0;
+    for (uint32_t w = 0; w < th >> 5; w++) at += part[w];
+    for (uint32_t i = r0; i < r1; i++) {
+        const Row y = row_at(i);
+        a.rows[i] = y, a.before[i] = at;
+        at += tiles_of(y) * y.parts;
+        if (y.parts > 1) cut = at;  // those come first
+        if (i + 1 == a.requests) a.head[1] = at * a.kv_heads;
+    }
+    if (few) {  // a request a thread
+        if (th == 0) sum = 0;
+        __syncthreads();
+        if (cut != 0) atomicMax(&sum, cut);
+        __syncthreads();
+        if (th == 0) a.head[0] = min(sum * a.kv_heads, a.blocks);
+    }
+}
+
 template <int D, int VD>
 __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const PrefillArgs a, uint32_t* status) {
     using S = Shape<D, VD>;
@@ -176,108 +297,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     extern __shared__ uint8_t raw_unaligned[];
     uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
     __shared__ Shared sh;
-    uint32_t* s_sum = reinterpret_cast<uint32_t*>(raw + S::OFF_Q);  // [requests + 1]: row tiles before each request
     const uint32_t th = threadIdx.x, warp = th >> 5, lane = th & 31;
     pdl_wait();
 
-    auto new_tokens = [&](uint32_t r, uint32_t& first) {
-        first = a.starts ? __ldg(a.starts + r) : r;
-        const uint32_t next = a.starts ? __ldg(a.starts + r + 1) : r + 1;
-        return next > first && first < a.tokens ? min(min(next - first, a.most), a.tokens - first) : 0u;
-    };
-    // The tiles of keys that a row tile sees: from position `from`, to before position `to`.
-    auto keys = [&](uint32_t row0, uint32_t n, int pos0, uint32_t& from, uint32_t& to) {
-        const int p_first = pos0 + (int)(row0 / a.ratio), p_last = pos0 + (int)min((row0 + ROWS - 1) / a.ratio, n - 1);
-        const int lowest = a.window != 0 && p_first >= (int)a.window ? p_first + 1 - (int)a.window : 0;
-        from = (uint32_t)lowest / KT * KT, to = p_last >= 0 ? (uint32_t)p_last + 1 : 0;
-        return to > from ? (to - from + KT - 1) / KT : 0u;
-    };
-    auto length = [&](uint32_t r) { return min(__ldg(a.lengths + r), a.width << a.shift); };
-    const bool few = a.requests <= FEW;
-    uint32_t most = 0xffffffffu;  // tiles of keys of a piece
-    if (few) {
-        if (th == 0) sh.work = 0;
-        __syncthreads();
-        uint32_t mine = 0;
-        if (th < a.requests) {
-            uint32_t first, from, to;
-            const uint32_t n = new_tokens(th, first), tiles = (n * a.ratio + ROWS - 1) / ROWS;
-            if (tiles != 0) {
-                mine = keys((tiles - 1) * ROWS, n, (int)length(th) - (int)n, from, to);
-                atomicAdd(&sh.work, (unsigned long long)mine * tiles * a.kv_heads);
-            }
-            sh.tiles[th] = mine;
-        }
-        __syncthreads();
-        if (th < a.requests) {
-            uint32_t rank = 0;
-            for (uint32_t o = 0; o < a.requests; o++) {
-                const uint32_t other = sh.tiles[o];
-                rank += other > mine || (other == mine && o < th);
-            }
-            sh.order[rank] = th;
-        }
-        most = (uint32_t)min(max((unsigned long long)LEAST, (sh.work + a.shares - 1) / a.shares), 0xffffffffull);
-        __syncthreads();
-    }
-    auto request = [&](uint32_t i) { return few ? sh.order[i] : i; };
-    auto parts_of = [&](uint32_t r) { return few ? max(1u, (sh.tiles[r] + most - 1) / most) : 1u; };
-    auto pieces = [&](uint32_t i) {
-        uint32_t first;
-        const uint32_t r = request(i);
-        return (new_tokens(r, first) * a.ratio + ROWS - 1) / ROWS * parts_of(r);
-    };
-    {  // pieces before each request
-        const uint32_t per = (a.requests + THREADS - 1) / THREADS, r0 = min(th * per, a.requests), r1 = min(r0 + per, a.requests);
-        uint32_t mine = 0;
-        for (uint32_t i = r0; i < r1; i++) mine += pieces(i);
-        uint32_t x = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= (uint32_t)o) x += y;
-        }
-        if (lane == 31) sh.part[warp] = x;
-        __syncthreads();
-        uint32_t at = x - mine;
-        for (uint32_t w = 0; w < warp; w++) at += sh.part[w];
-        for (uint32_t i = r0; i < r1; i++) {
-            s_sum[i] = at;
-            at += pieces(i);
-            if (i + 1 == a.requests) s_sum[a.requests] = at;
-        }
-        __syncthreads();
-    }
-    const uint32_t items = s_sum[a.requests];
-    if (few && blockIdx.x == 0 && blockIdx.y == 0 && th == 0) {
-        uint32_t i = 0;
-        while (i < a.requests && parts_of(request(i)) > 1) i++;
-        *a.cut = min(s_sum[i] * a.kv_heads, gridDim.x);
-    }
-    if (blockIdx.x >= items * a.kv_heads) return;
-    uint32_t i_req = 0;
-    {
+    if (blockIdx.x >= a.head[1]) return;
+    if (warp == MMA_WARP + 1) {  // the block's request: 32 places at once
         const uint32_t item = blockIdx.x / a.kv_heads;
-        uint32_t hi = a.requests;
-        while (hi - i_req > 1) {
-            const uint32_t mid = (i_req + hi) >> 1;
-            if (s_sum[mid] <= item) i_req = mid;
-            else hi = mid;
+        uint32_t lo = 0, start = 0;
+        for (uint32_t step = (a.requests + 31) / 32;; step = (step + 31) / 32) {
+            const uint32_t at = lo + lane * step, before = at < a.requests ? a.before[at] : 0xffffffffu;
+            const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, before <= item));
+            lo += last * step, start = __shfl_sync(0xffffffffu, before, last);
+            if (step == 1) break;
         }
+        if (lane == 0) sh.row = a.rows[lo], sh.place = item - start;
     }
-    // A request's last rows, which see most, first; a row tile's pieces behind one another.
-    const uint32_t r = request(i_req), kvh = blockIdx.x % a.kv_heads, parts = parts_of(r);
-    uint32_t first, tile0, end;
-    const uint32_t n = new_tokens(r, first), place = blockIdx.x / a.kv_heads - s_sum[i_req], part = place % parts;
-    const uint32_t row0 = ((n * a.ratio + ROWS - 1) / ROWS - 1 - place / parts) * ROWS;
-    const int pos0 = (int)length(r) - (int)n;  // the first new token's position; negative when the lengths cannot be
-    uint32_t nt = keys(row0, n, pos0, tile0, end);
-    if (parts > 1) {
-        const uint32_t each = (nt + parts - 1) / parts, t0 = min(part * each, nt);
-        nt = min(each, nt - t0), tile0 += t0 * KT;
-        if (th == 0 && blockIdx.y == 0) a.splits[blockIdx.x] = Split{part == 0 ? parts : 0, row0, kvh, first, n};
-    }
-
     if (th == 0) {
         mbar_init(&sh.q_full, SOFT_WARPS), mbar_init(&sh.drained, 1);
         for (int i = 0; i < 2; i++) mbar_init(&sh.k_full[i], GROUP_WARPS), mbar_init(&sh.v_full[i], GROUP_WARPS), mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_ready[i], SOFT_WARPS);
@@ -293,6 +327,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prefill_kernel(const Prefill
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sh.tmem;
+    // A request's last rows, which see most, first; a row tile's pieces behind one another.
+    const uint32_t r = sh.row.r, kvh = blockIdx.x % a.kv_heads, parts = sh.row.parts, first = sh.row.first, n = sh.row.n, part = sh.place % parts;
+    const uint32_t row0 = ((n * a.ratio + ROWS - 1) / ROWS - 1 - sh.place / parts) * ROWS;
+    const int pos0 = (int)sh.row.len - (int)n;  // the first new token's position; negative when the lengths cannot be
+    uint32_t tile0, end, nt = keys_of<KT>(a, row0, n, pos0, tile0, end);
+    if (parts > 1) {
+        const uint32_t each = (nt + parts - 1) / parts, t0 = min(part * each, nt);
+        nt = min(each, nt - t0), tile0 += t0 * KT;
+        if (th == 0 && blockIdx.y == 0) a.splits[blockIdx.x] = Split{part == 0 ? parts : 0, row0, kvh, first, n};
+    }
     bool ok = true;
     // A wait that runs out is noted, and the thread goes on without waiting for anything else.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -658,7 +702,7 @@ template <int D, int VD>
 __global__ void __launch_bounds__(ROWS) paged_prefill_join_kernel(const PrefillArgs a) {
     const uint32_t row = threadIdx.x, col = blockIdx.y * 16;
     pdl_wait();
-    const uint32_t cut = *a.cut;
+    const uint32_t cut = a.head[0];
     for (uint32_t b = blockIdx.x; b < cut; b += gridDim.x) {
         const Split s = a.splits[b];
         const uint32_t at = s.row0 + row, tok = at / a.ratio, head = s.kvh * a.ratio + at % a.ratio;
@@ -709,17 +753,17 @@ uint32_t shares_of(const tb_context* ctx, uint32_t head_dim) { return std::max((
 template <int D, int VD>
 int run(tb_context* ctx, const PrefillArgs& a, uint32_t grid) {
     static std::atomic<uint64_t> done{0};
-    using S = Shape<D, VD>;
-    constexpr size_t bytes = 1024 + S::OFF_Q + std::max<size_t>(ROWS * S::Q_ROW, (MAX_REQUESTS + 1) * 4);
+    constexpr size_t bytes = Shape<D, VD>::BYTES;
     static_assert(bytes + sizeof(Shared) <= 232448, "over what a block may use");
     TB_CUDA(allow_smem(paged_prefill_kernel<D, VD>, bytes, ctx->gpu, done));
+    TB_CUDA(launch_kernel(ctx, paged_prefill_plan_kernel<Shape<D, VD>::KT>, dim3(1), dim3(THREADS), 0, true, a));
     TB_CUDA(launch_kernel(ctx, paged_prefill_kernel<D, VD>, dim3(grid, D / VD), dim3(THREADS), bytes, true, a, ctx->status));
     if (a.requests <= FEW) TB_CUDA(launch_kernel(ctx, paged_prefill_join_kernel<D, VD>, dim3(a.shares, VD / 16, D / VD), dim3(ROWS), 0, true, a));
     return OK;
 }
 
-// The scratch: the decode kernel's counters, which stay zero; how many pieces; what they are of; the pieces.
-constexpr size_t SPLITS_AT = PAGED_COUNT_BYTES + 16;
+// The scratch: the decode kernel's counters, which stay zero; `head`, `before`, `rows`, `splits`; the pieces.
+constexpr size_t BEFORE_AT = PAGED_COUNT_BYTES + 16, ROWS_AT = BEFORE_AT + MAX_REQUESTS * 4, SPLITS_AT = ROWS_AT + MAX_REQUESTS * sizeof(Row);
 size_t partial_at(uint32_t shares) { return SPLITS_AT + ((size_t)2 * shares * sizeof(Split) + 15) / 16 * 16; }
 
 }  // namespace
@@ -741,10 +785,12 @@ int launch_prefill_paged(tb_context* ctx, const tb_paged_attend& p) {
     const uint64_t full = (uint64_t)p.tokens * a.ratio / ROWS + c.requests, each = (((uint64_t)p.most * a.ratio + ROWS - 1) / ROWS) * c.requests;
     a.shares = shares_of(ctx, c.head_dim);
     const uint64_t grid = (full < each ? full : each) * c.kv_heads + (c.requests <= FEW ? a.shares : 0);  // cutting makes at most as many more
+    a.blocks = (uint32_t)grid;
     if (grid > 0x7fffffffull) return fail(OUT_OF_RANGE, "tb_prefill_paged_q8: too many rows for one call");
     TB_TRY(check_scratch(ctx, p, "tb_prefill_paged_q8"));
     uint8_t* scratch = static_cast<uint8_t*>(p.scratch);
-    a.cut = reinterpret_cast<uint32_t*>(scratch + PAGED_COUNT_BYTES), a.splits = reinterpret_cast<Split*>(scratch + SPLITS_AT);
+    a.head = reinterpret_cast<uint32_t*>(scratch + PAGED_COUNT_BYTES), a.before = reinterpret_cast<uint32_t*>(scratch + BEFORE_AT);
+    a.rows = reinterpret_cast<Row*>(scratch + ROWS_AT), a.splits = reinterpret_cast<Split*>(scratch + SPLITS_AT);
     a.partial = reinterpret_cast<float*>(scratch + partial_at(a.shares));
     DeviceScope scope(ctx->gpu);
     TB_CUDA(scope.error());
