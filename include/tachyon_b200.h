@@ -410,7 +410,7 @@ typedef struct tb_plan {
     uint32_t* slots;       /* [max_tokens] */
     uint32_t* positions;   /* [max_tokens] or NULL */
     uint32_t* refused;
-    uint32_t* scratch;     /* one word, zero before the first launch, left zero */
+    uint32_t* scratch;     /* one word, zero before the first launch, left zero; not for calls that overlap */
     uint32_t requests, width, page, pages, max_tokens;
 } tb_plan;
 TB_API int tb_page_plan(tb_context* ctx, const tb_plan* args);
@@ -477,7 +477,7 @@ TB_API int tb_prefill_paged_q8(tb_context* ctx, const tb_paged_attend* args);
  *   c = its count in history[r][prompt[r] .. total[r]): x -= c > 0 ? frequency[r] * c + presence[r] : 0
  *   bias_token[r][i] == t, i < bias_count[r]:        x += bias[r][i], in the order of i (summed first when a token comes twice)
  *   mask m = mask_of[r] (NULL: r), bit t clear:      x = -inf (also over NaN); m >= masks: no mask.  A mask may let nothing through: the row is -inf.
- * f32 arithmetic, rounded once to dtype.  Tokens past the vocabulary in history and biases are ignored.  out may be logits.
+ * f32 arithmetic (x / repetition is x times the rounded 1 / repetition, both normal numbers), rounded once to dtype.  Tokens past the vocabulary in history and biases are ignored.  out may be logits.
  */
 typedef struct tb_logits {
     const void* logits;    /* [rows][vocab], stride values from row to row */

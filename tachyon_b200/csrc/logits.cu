@@ -12,7 +12,7 @@
 // whose tokens has a word only masks them.  Every block of a row walks all of its history, so ranges are as long as leaves three blocks a
 // multiprocessor, for a small batch shorter.  Measured slower: clusters that share the walk and count in each other's shared memory;
 // the few tokens with words worked out one by one; a kernel of their own for those with hashed tables (64 rows of 262144 in f16 with 8000
-// tokens of history: 53 us, 13 of them the stream).
+// tokens of history: 53 us, 13 of them the stream; this one 33, and 3.3 for one row in f32 with 2000).
 #include "common.cuh"
 #include "paged.h"
 

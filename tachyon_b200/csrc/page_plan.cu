@@ -9,6 +9,8 @@
 //
 // Every block repeats the prefix sum (8 bytes a request from the L2) and takes its share of the tokens and pages, finding a
 // token's request by bisection in shared memory; a second launch behind a scan of one block would cost more than the repeats.
+// What bounds it: trips to memory one behind the other (lengths, table entries).  64 single tokens 5 us, an empty launch being 2.5; 1000
+// requests that bring up to 257 tokens each 8.7 us (with 4096 tokens a block instead of 1024: 15.5).
 #include "common.cuh"
 #include "paged.h"
 

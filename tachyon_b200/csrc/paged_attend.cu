@@ -18,6 +18,11 @@
 //   O^T = V^T P^T: the scores' accumulator is the B operand's layout as it stands; the weights again go in two f16 parts.  A page's
 //   value scale multiplies the weights, relative to the largest scale met so far, so they stay within f16.
 // Softmax statistics and sums are f32.
+//
+// Measured: 96 requests of up to 16384 positions, 32 query heads on 8 of 128, 1.12 GB: 235 us, 4.8 TB/s or 73 % of a copy's rate; 446
+// instructions for 16 positions keep the schedulers 59 % busy, the rest is the conversion's latency.  Two requests of up to 131071
+// positions, heads of 512: 103 us (3.7 TB/s; registers and rings leave one block a multiprocessor).  One request of 4096 positions 13 us, 33
+// with a window of 512 17 us: the trips to the lengths, the page table, the scales and the codes, and code that is met for the first time.
 #include <algorithm>
 
 #include "common.cuh"

@@ -593,6 +593,38 @@ def test_prefill_gives_the_same_bits_and_shares_scratch(ctx):
         assert np.array_equal(a, b)
 
 
+def test_two_contexts_at_once(ctx):
+    """Two streams over the same cache, each with its own scratch, nothing waited for in between."""
+    other = tb.Context(0)
+    D, kvh, ratio, page = 128, 2, 4, 64
+    cache = Cache(ctx, 80, kvh, page, D, 1)
+    rng = np.random.default_rng(8)
+    lengths, new = [5000, 700, 31], [70, 1, 31]
+    table = words(ctx, tables(rng, lengths, page, 80, 80))
+    starts, lens = words(ctx, np.concatenate([[0], np.cumsum(new)])), words(ctx, lengths)
+    tokens, row = sum(new), kvh * ratio * D
+    q = ctx.upload(rng.standard_normal((tokens, row)).astype(np.float16))
+    ctx.sync()
+    outs = []
+    for c in (ctx, other):
+        for prefill in (True, False):
+            scratch = c.zeros(c.paged_scratch_bytes(D))
+            most = max(new) if prefill else 2
+            outs.append((c, prefill, [c.zeros(tokens * row * 4) for _ in range(6)], scratch, most))
+        c.sync()
+    for i in range(6):
+        for c, prefill, out, scratch, most in outs:
+            a = tb.PagedAttend(cache=cache.pages_of(table, 3, 80), q=q.ptr, q_dtype=tb.F16, q_stride=row, starts=starts.ptr, lengths=lens.ptr, tokens=tokens,
+                               heads=kvh * ratio, most=most, window=0, scale=0.1, out=out[i].ptr, out_dtype=tb.F32, out_stride=row, scratch=scratch.ptr,
+                               scratch_bytes=scratch.nbytes)
+            (c.prefill_paged_q8 if prefill else c.attend_paged_q8)(a)
+    got = [[o.download(np.uint32, tokens * row) for o in out] for _, _, out, _, _ in outs]
+    for k in range(4):
+        for x in got[k]:
+            assert np.array_equal(x, got[k % 2][0])
+    assert got[0][0].any() and got[1][0].any()
+
+
 def test_prefill_needs_its_scratch(ctx):
     cache = Cache(ctx, 2, 1, 16, 64, 1)
     small = ctx.zeros(ctx.paged_scratch_bytes(64) - 16)
