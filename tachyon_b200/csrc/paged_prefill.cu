@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(THREADS) paged_prefill_plan_kernel(const Prefi
     if (few) {
         if (th == 0) work = 0;
         __syncthreads();
+        unsigned long long product = 0;
         uint32_t mine = 0, tiles = 0;  // tiles of keys of a request's last row tile, which sees most; its row tiles
         if (th < a.requests) {
             uint32_t from, to;
@@ -235,10 +236,12 @@ __global__ void __launch_bounds__(THREADS) paged_prefill_plan_kernel(const Prefi
             tiles = tiles_of(x);
             if (tiles != 0) {
                 mine = keys_of<KT>(a, (tiles - 1) * ROWS, x.n, (int)x.len - (int)x.n, from, to);
-                atomicAdd(&work, (unsigned long long)mine * tiles * a.kv_heads);
+                product = (unsigned long long)mine * tiles * a.kv_heads;
             }
             seen[th] = mine;
         }
+        for (int o = 16; o != 0; o >>= 1) product += __shfl_xor_sync(0xffffffffu, product, o);  // by lanes each for itself: 64-bit atomics on one word, 6 us
+        if (lane == 0 && product != 0) atomicAdd(&work, product);
         __syncthreads();
         if (th < a.requests) {
             uint32_t rank = 0;
